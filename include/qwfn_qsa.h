@@ -93,9 +93,11 @@ extern "C" {
 #define QWFN_KV_Q4_0  1
 #define QWFN_KV_F16   2
 
-/* element type of K/V rows handed to the append */
+/* element type of K/V rows handed to the append; BF16 rows are taken by the
+ * rotary and window calls only */
 #define QWFN_SRC_F32  0
 #define QWFN_SRC_F16  1
+#define QWFN_SRC_BF16 2
 
 /* bits of view->status */
 #define QWFN_STATUS_POS_RANGE    0x1  /* a position >= the view's capacity     */
@@ -434,6 +436,113 @@ int qwfn_sparse_attn_prefill(const qwfn_qsa_shape *shape, const qwfn_kv_view *vi
                              int32_t src_dtype, int32_t seq, int32_t pos0, int32_t n_q,
                              float *out, int32_t *sel_out, int32_t *n_sel_out,
                              int32_t max_sel, void *ws, size_t ws_bytes, void *stream);
+
+/* ---- rotary positions ------------------------------------------------------ */
+/* The caller's side of the layer norms and turns Q and K before they reach the
+ * calls above (src/qwfn_graph.cpp:244-254, 463-470, 480-484 for the indexer's;
+ * the layer's own projections alike).  These calls do that: to rows anywhere
+ * (qwfn_rope_rows: queries, the checkpoint indexer's q_idx and raw keys), or to
+ * a token's K on its way into the cache (qwfn_kv_append_rope).
+ *
+ * A head row x of head_dim values, at position p:
+ *   norm    (given fp32 weights w [head_dim]) z_d = x_d w_d / sqrt(mean_d(x_d^2)
+ *           + norm_eps); else z = x
+ *   rotary  pair i of the first rope_dim values, (i, i + rope_dim/2) (HALF) or
+ *           (2i, 2i+1) (INTERLEAVED), turns by 2 pi p turns[i]:
+ *           (a, b) -> mscale (a cos - b sin, b cos + a sin); the others pass
+ *   result  evaluated in 64 bits, rounded once to fp32, then to the row's type
+ *           or, for K, quantized as qwfn_kv_append_q8_0 does.
+ * turns holds the frequencies over 2 pi, so position scaling for long contexts
+ * is a matter of the table (qwfnfer_amd.qsa.RopeConfig fills it for linear and
+ * YaRN scaling; mscale is YaRN's factor).  The reference's IMROPE with equal
+ * sections, as for text, is HALF.  Its angle is an fp32 chain (see the indexer
+ * keys below), this one the exact product: at position p they differ by up to
+ * about p * 2^-23 radians in the fastest pairs.                                */
+#define QWFN_ROPE_HALF         0
+#define QWFN_ROPE_INTERLEAVED  1
+typedef struct qwfn_rope {
+    int32_t       rope_dim;  /* rotated values of a head row: even, >= 2         */
+    int32_t       layout;    /* QWFN_ROPE_*                                      */
+    const double *turns;     /* [rope_dim / 2] turns a position, device          */
+    float         mscale;    /* factor on cos and sin (1: none)                  */
+    float         norm_eps;  /* of the norm, where its weights are given         */
+} qwfn_rope;
+/* Head rows: value d of row r's head h is at data + (r * row_stride + h *
+ * head_stride + d) elements of dtype (QWFN_SRC_*), as rows lie in a fused
+ * projection's output.  Strides are in elements and not negative.  Data is
+ * aligned to its element; 16-byte aligned rows (pointer and strides) are
+ * faster.                                                                      */
+typedef struct qwfn_rows {
+    void    *data;
+    int32_t  dtype;
+    int64_t  row_stride, head_stride;
+} qwfn_rows;
+/* Norm (norm != NULL: fp32 [head_dim]) and turn n_rows x n_heads head rows of
+ * src at pos[r] (device, any int32) into dst.  inverse != 0 turns the other
+ * way: the transpose of the rotation (over mscale^2, its inverse), which is also the
+ * gradient of unnormed rows.  head_dim 1 .. 512, rope_dim <= head_dim.  dst is src itself (same
+ * pointer, type and strides) or apart from it: QWFN_EINVAL when they overlap
+ * otherwise.  Head rows of dst must not overlap each other.                    */
+int qwfn_rope_rows(const qwfn_rope *rope, const qwfn_rows *src, const float *norm, const int32_t *pos,
+                   int32_t n_rows, int32_t n_heads, int32_t head_dim, int32_t inverse, const qwfn_rows *dst,
+                   void *stream);
+/* qwfn_kv_append_q8_0 with the rotation on the way: row r's K (normed when
+ * k_norm is given, and turned at pos[r]) and V (as it is) go to (seq_ids[r] or
+ * 0, pos[r]) in the view's cache type.  With q != NULL the row's n_head query
+ * heads are normed (q_norm) and turned in the same launch into q_out, which
+ * does not overlap any source.  Pooled keys are left alone, as by
+ * qwfn_kv_append_q8_0: pool the blocks the rows complete (qwfn_pool_update).
+ * A bad sequence, position or page skips the row's K and V and sets its status
+ * bit; q_out is written all the same.  Rows of one call with the same
+ * (sequence, position) leave unspecified bytes there.                          */
+int qwfn_kv_append_rope(const qwfn_qsa_shape *shape, const qwfn_kv_view *view, const qwfn_rope *rope,
+                        const qwfn_rows *k, const qwfn_rows *v, const float *k_norm, const int32_t *seq_ids,
+                        const int32_t *pos, int32_t n_rows, const qwfn_rows *q, const float *q_norm,
+                        const qwfn_rows *q_out, void *stream);
+
+/* ---- sliding-window attention ---------------------------------------------- */
+/* Attention over the cache with a sliding window and a few first tokens that
+ * stay visible, exact to the token (the selection's local_tokens and
+ * sink_blocks keep whole blocks): the query at position p of a sequence sees
+ * the cells t <= p with t > p - window or t < sink_tokens, scale
+ * 1/sqrt(head_dim).  The selection fields and kv_round_f16 of the shape are not
+ * used, nor are pooled keys.  q and out are [rows][n_head][head_dim] of one
+ * dtype (QWFN_SRC_*), 16-byte aligned and apart from each other; sums, maxima and weights are held in
+ * fp32.  F32 and F16 rows are computed from the exact cached values to fp32
+ * rounding; for BF16 rows the operands of the products are rounded to fp16.
+ *
+ * Pages wholly outside the window and the first tokens are not read, so their
+ * page-table entries may hold anything, -1 for pages given back.  A visible
+ * page outside the pool sets QWFN_STATUS_PAGE_RANGE and its cells are not
+ * attended.  A cell that a query does not see does not change its result,
+ * whatever it holds; a NaN or infinity that it sees makes its output (from V:
+ * that value of it) NaN or infinite.
+ * n_head / n_head_kv is at most 16 (QWFN_ENOTSUP).                             */
+
+/* Workspace of the two calls for up to n_seq sequences, n_rows query rows of
+ * dtype, max_q of one sequence and max_seq_len tokens (n_rows = n_seq, max_q =
+ * 1: decode only).  It needs no initialisation and holds nothing between
+ * calls; calls that overlap on one workspace race.                             */
+int qwfn_window_workspace_bytes(const qwfn_qsa_shape *shape, int32_t n_seq, int32_t n_rows, int32_t max_q,
+                                int32_t max_seq_len, int32_t window, int32_t sink_tokens, int32_t dtype,
+                                size_t *bytes);
+/* One query a sequence, at position seq_len[s] - 1 (seq_len on the device).
+ * A sequence of length 0 (a padded row) gets a zero row.  Lengths outside
+ * [0, max_seq_len] set QWFN_STATUS_LEN_RANGE and get one too.                  */
+int qwfn_window_attn_decode(const qwfn_qsa_shape *shape, const qwfn_kv_view *view, const void *q, int32_t dtype,
+                            const int32_t *seq_len, int32_t n_seq, int32_t max_seq_len, int32_t window,
+                            int32_t sink_tokens, void *out, void *ws, size_t ws_bytes, void *stream);
+/* Queries of several sequences in one call: rows [q_start[s], q_start[s + 1])
+ * are the last ones of sequence s, whose length with them is seq_len[s]
+ * (device; q_start ascends within [0, n_rows]).  Their K and V are in the cache
+ * already.  n_rows is the number of rows of q and out, max_q a bound on one
+ * sequence's queries.  Rows outside every sequence are left as they were.  A
+ * sequence of more queries than tokens or than max_q, or of a length outside
+ * [0, max_seq_len], sets QWFN_STATUS_LEN_RANGE and gets zero rows.             */
+int qwfn_window_attn_prefill(const qwfn_qsa_shape *shape, const qwfn_kv_view *view, const void *q, int32_t dtype,
+                             const int32_t *q_start, const int32_t *seq_len, int32_t n_seq, int32_t n_rows,
+                             int32_t max_q, int32_t max_seq_len, int32_t window, int32_t sink_tokens, void *out,
+                             void *ws, size_t ws_bytes, void *stream);
 
 /* ---- the checkpoint's own indexer ---------------------------------------- */
 /* The released checkpoint scores blocks with a separate indexer

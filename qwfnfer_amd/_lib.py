@@ -22,6 +22,9 @@ KV_Q4_0 = 1
 KV_F16 = 2
 SRC_F32 = 0
 SRC_F16 = 1
+SRC_BF16 = 2                    # rotary and window calls only
+ROPE_HALF = 0
+ROPE_INTERLEAVED = 1
 
 STATUS_POS_RANGE = 0x1
 STATUS_SEQ_RANGE = 0x2
@@ -66,6 +69,11 @@ EXPORTS = (
     "qwfn_idx_select",
     "qwfn_idx_sparse_attn_decode",
     "qwfn_idx_sparse_attn_prefill",
+    "qwfn_rope_rows",
+    "qwfn_kv_append_rope",
+    "qwfn_window_workspace_bytes",
+    "qwfn_window_attn_decode",
+    "qwfn_window_attn_prefill",
 )
 
 
@@ -119,6 +127,25 @@ class IdxView(C.Structure):
     ]
 
 
+class RopeStruct(C.Structure):
+    _fields_ = [
+        ("rope_dim", C.c_int32),
+        ("layout", C.c_int32),
+        ("turns", C.c_void_p),
+        ("mscale", C.c_float),
+        ("norm_eps", C.c_float),
+    ]
+
+
+class RowsStruct(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("dtype", C.c_int32),
+        ("row_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+    ]
+
+
 class QsaError(RuntimeError):
     """A negative return code of the C ABI, with qwfn_qsa_last_error()."""
 
@@ -134,6 +161,8 @@ _S = C.POINTER(QsaShape)
 _V = C.POINTER(KvView)
 _IS = C.POINTER(IdxShape)
 _IV = C.POINTER(IdxView)
+_R = C.POINTER(RopeStruct)
+_RW = C.POINTER(RowsStruct)
 _P = C.c_void_p
 _I = C.c_int32
 _Z = C.c_size_t
@@ -176,6 +205,11 @@ _SIGS = {
                                               _P, _Z, _P]),
     "qwfn_idx_sparse_attn_prefill": (C.c_int, [_S, _V, _IS, _IV, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P,
                                                _I, _P, _Z, _P]),
+    "qwfn_rope_rows": (C.c_int, [_R, _RW, _P, _P, _I, _I, _I, _I, _RW, _P]),
+    "qwfn_kv_append_rope": (C.c_int, [_S, _V, _R, _RW, _RW, _P, _P, _P, _I, _RW, _P, _RW, _P]),
+    "qwfn_window_workspace_bytes": (C.c_int, [_S, _I, _I, _I, _I, _I, _I, _I, C.POINTER(_Z)]),
+    "qwfn_window_attn_decode": (C.c_int, [_S, _V, _P, _I, _P, _I, _I, _I, _I, _P, _P, _Z, _P]),
+    "qwfn_window_attn_prefill": (C.c_int, [_S, _V, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _Z, _P]),
 }
 
 

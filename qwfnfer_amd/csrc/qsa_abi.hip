@@ -1143,4 +1143,200 @@ int qwfn_idx_sparse_attn_prefill(const qwfn_qsa_shape *shape, const qwfn_kv_view
                         max_sel, ws, ws_bytes, stream);
 }
 
+// ---- rotary positions ----
+
+static size_t dtype_size(int32_t t) { return t == QWFN_SRC_F32 ? 4 : 2; }
+
+static int check_dtype(const char *what, int32_t t) {
+    if (t != QWFN_SRC_F32 && t != QWFN_SRC_F16 && t != QWFN_SRC_BF16)
+        return fail(QWFN_EINVAL, "%s: dtype %d unknown", what, t);
+    return QWFN_OK;
+}
+
+static int make_rope(const char *what, const qwfn_rope *r, int32_t head_dim, int32_t inverse, RopeArg *out) {
+    if (!r) return fail(QWFN_EINVAL, "%s: rope is NULL", what);
+    if (r->rope_dim < 2 || r->rope_dim % 2 || r->rope_dim > head_dim)
+        return fail(QWFN_EINVAL, "%s: rope_dim %d is not an even number in [2, head_dim %d]", what, r->rope_dim, head_dim);
+    if (r->layout != QWFN_ROPE_HALF && r->layout != QWFN_ROPE_INTERLEAVED)
+        return fail(QWFN_EINVAL, "%s: rope layout %d unknown", what, r->layout);
+    if (!r->turns || !aligned(r->turns, 8)) return fail(QWFN_EINVAL, "%s: turns NULL or not 8-byte aligned", what);
+    if (!std::isfinite(r->mscale) || !std::isfinite(r->norm_eps) || r->norm_eps < 0.0f)
+        return fail(QWFN_EINVAL, "%s: mscale or norm_eps not finite, or norm_eps < 0", what);
+    *out = RopeArg{r->turns, r->rope_dim, r->layout == QWFN_ROPE_INTERLEAVED, inverse != 0, r->mscale, r->norm_eps};
+    return QWFN_OK;
+}
+
+// Elements from the first value of n_rows x heads head rows to past the last.
+static int64_t rows_extent(const RowsArg &r, int32_t n_rows, int32_t heads, int32_t hd) {
+    return (int64_t)(n_rows - 1) * r.row_stride + (int64_t)(heads - 1) * r.head_stride + hd;
+}
+
+static int make_rows(const char *what, const qwfn_rows *r, int32_t n_rows, int32_t heads, int32_t hd, RowsArg *out) {
+    if (!r || !r->data) return fail(QWFN_EINVAL, "%s is NULL", what);
+    const int rc = check_dtype(what, r->dtype);
+    if (rc) return rc;
+    if (!aligned(r->data, dtype_size(r->dtype))) return fail(QWFN_EINVAL, "%s is not aligned to its type", what);
+    if (r->row_stride < 0 || r->head_stride < 0 || r->row_stride > INT64_MAX / 16 / n_rows ||
+        r->head_stride > INT64_MAX / 16 / heads)
+        return fail(QWFN_EINVAL, "%s: strides %lld, %lld negative or too large", what, (long long)r->row_stride,
+                    (long long)r->head_stride);
+    (void)hd;
+    *out = RowsArg{r->data, r->dtype, r->row_stride, r->head_stride};
+    return QWFN_OK;
+}
+
+// dst's head rows must be apart from each other.
+static int check_dst(const char *what, const RowsArg &r, int32_t n_rows, int32_t heads, int32_t hd) {
+    const int64_t a = std::min(r.row_stride, r.head_stride), b = std::max(r.row_stride, r.head_stride);
+    const int64_t na = r.row_stride <= r.head_stride ? n_rows : heads;      // of the smaller stride
+    const int64_t nb = r.row_stride <= r.head_stride ? heads : n_rows;
+    if ((na > 1 && a < hd) || (nb > 1 && b < (na > 1 ? a * (na - 1) : 0) + hd))
+        return fail(QWFN_EINVAL, "%s: head rows overlap (strides %lld, %lld)", what, (long long)r.row_stride,
+                    (long long)r.head_stride);
+    return QWFN_OK;
+}
+
+static bool overlap(const RowsArg &a, int32_t heads_a, const RowsArg &b, int32_t heads_b, int32_t n_rows, int32_t hd) {
+    const uintptr_t a0 = (uintptr_t)a.data, b0 = (uintptr_t)b.data;
+    return a0 < b0 + (uintptr_t)rows_extent(b, n_rows, heads_b, hd) * dtype_size(b.dtype) &&
+           b0 < a0 + (uintptr_t)rows_extent(a, n_rows, heads_a, hd) * dtype_size(a.dtype);
+}
+
+int qwfn_rope_rows(const qwfn_rope *rope, const qwfn_rows *src, const float *norm, const int32_t *pos,
+                   int32_t n_rows, int32_t n_heads, int32_t head_dim, int32_t inverse, const qwfn_rows *dst,
+                   void *stream) {
+    if (n_rows < 1 || n_heads < 1) return fail(QWFN_EINVAL, "rope_rows: n_rows %d or n_heads %d < 1", n_rows, n_heads);
+    if (head_dim < 1 || head_dim > kRopeMaxDim)
+        return fail(QWFN_EINVAL, "rope_rows: head_dim %d outside [1, %d]", head_dim, kRopeMaxDim);
+    if ((int64_t)n_rows * n_heads > INT32_MAX)
+        return fail(QWFN_ERANGE, "rope_rows: more than %d head rows", INT32_MAX);
+    RopeArg rp;
+    RowsArg s, d;
+    int rc;
+    if ((rc = make_rope("rope_rows", rope, head_dim, inverse, &rp)) ||
+        (rc = make_rows("rope_rows: src", src, n_rows, n_heads, head_dim, &s)) ||
+        (rc = make_rows("rope_rows: dst", dst, n_rows, n_heads, head_dim, &d)) ||
+        (rc = check_dst("rope_rows: dst", d, n_rows, n_heads, head_dim)))
+        return rc;
+    if (!pos || !aligned(pos, 4) || !aligned(norm, 4)) return fail(QWFN_EINVAL, "rope_rows: pos NULL, or pos or norm misaligned");
+    const bool same = s.data == d.data && s.dtype == d.dtype && s.row_stride == d.row_stride && s.head_stride == d.head_stride;
+    if (!same && overlap(s, n_heads, d, n_heads, n_rows, head_dim))
+        return fail(QWFN_EINVAL, "rope_rows: dst overlaps src and is not src itself");
+    const hipError_t e = launch_rope_rows(rp, s, norm, pos, n_rows, n_heads, head_dim, d, (hipStream_t)stream);
+    return e == hipSuccess ? ok() : hip_fail(e, "rope_rows");
+}
+
+int qwfn_kv_append_rope(const qwfn_qsa_shape *shape, const qwfn_kv_view *view, const qwfn_rope *rope,
+                        const qwfn_rows *k, const qwfn_rows *v, const float *k_norm, const int32_t *seq_ids,
+                        const int32_t *pos, int32_t n_rows, const qwfn_rows *q, const float *q_norm,
+                        const qwfn_rows *q_out, void *stream) {
+    Geo g;
+    int rc = make_geo(shape, view, &g);
+    if (rc) return rc;
+    if (n_rows < 1) return fail(QWFN_EINVAL, "append_rope: n_rows %d < 1", n_rows);
+    if ((int64_t)n_rows * (g.H + 2 * g.Hkv) > INT32_MAX)
+        return fail(QWFN_ERANGE, "append_rope: more than %d head rows", INT32_MAX);
+    RopeArg rp;
+    RowsArg ka, va, qa{nullptr, 0, 0, 0}, qo{nullptr, 0, 0, 0};
+    if ((rc = make_rope("append_rope", rope, g.hd, 0, &rp)) ||
+        (rc = make_rows("append_rope: k", k, n_rows, g.Hkv, g.hd, &ka)) ||
+        (rc = make_rows("append_rope: v", v, n_rows, g.Hkv, g.hd, &va)))
+        return rc;
+    if (!pos || !aligned(pos, 4) || !aligned(seq_ids, 4) || !aligned(k_norm, 4) || !aligned(q_norm, 4))
+        return fail(QWFN_EINVAL, "append_rope: pos NULL, or pos, seq_ids or a norm misaligned");
+    if ((q == nullptr) != (q_out == nullptr))
+        return fail(QWFN_EINVAL, "append_rope: q and q_out come together");
+    if (!q && q_norm) return fail(QWFN_EINVAL, "append_rope: q_norm without q");
+    if (q) {
+        if ((rc = make_rows("append_rope: q", q, n_rows, g.H, g.hd, &qa)) ||
+            (rc = make_rows("append_rope: q_out", q_out, n_rows, g.H, g.hd, &qo)) ||
+            (rc = check_dst("append_rope: q_out", qo, n_rows, g.H, g.hd)))
+            return rc;
+        if (overlap(qo, g.H, qa, g.H, n_rows, g.hd) || overlap(qo, g.H, ka, g.Hkv, n_rows, g.hd) ||
+            overlap(qo, g.H, va, g.Hkv, n_rows, g.hd))
+            return fail(QWFN_EINVAL, "append_rope: q_out overlaps a source");
+    }
+    const hipError_t e = launch_rope_append(g, *view, rp, qa, ka, va, q_norm, k_norm, seq_ids, pos, n_rows, qo,
+                                            (hipStream_t)stream);
+    return e == hipSuccess ? ok() : hip_fail(e, "append_rope");
+}
+
+// ---- sliding-window attention ----
+
+static int check_window(const char *what, const Geo &g, const WinPlan &p) {
+    int rc = check_dtype(what, p.dtype);
+    if (rc) return rc;
+    if (g.G > 16) return fail(QWFN_ENOTSUP, "%s: %d query heads a KV head, at most 16", what, g.G);
+    if (p.window < 1) return fail(QWFN_EINVAL, "%s: window %d < 1", what, p.window);
+    if (p.sinks < 0) return fail(QWFN_EINVAL, "%s: sink_tokens %d < 0", what, p.sinks);
+    if (p.n_seq < 1 || p.n_rows < 1 || p.max_q < 1 || p.max_seq_len < 1)
+        return fail(QWFN_EINVAL, "%s: n_seq %d, n_rows %d, max_q %d or max_seq_len %d < 1", what, p.n_seq, p.n_rows,
+                    p.max_q, p.max_seq_len);
+    if (p.max_seq_len > INT32_MAX / 2) return fail(QWFN_ERANGE, "%s: max_seq_len %d", what, p.max_seq_len);
+    if ((int64_t)p.n_seq * g.Hkv > kMaxCounters)
+        return fail(QWFN_ERANGE, "%s: n_seq * n_head_kv = %lld exceeds %d", what, (long long)p.n_seq * g.Hkv, kMaxCounters);
+    if ((int64_t)p.n_rows * g.H > INT32_MAX) return fail(QWFN_ERANGE, "%s: n_rows * n_head exceeds %d", what, INT32_MAX);
+    return QWFN_OK;
+}
+
+int qwfn_window_workspace_bytes(const qwfn_qsa_shape *shape, int32_t n_seq, int32_t n_rows, int32_t max_q,
+                                int32_t max_seq_len, int32_t window, int32_t sink_tokens, int32_t dtype,
+                                size_t *bytes) {
+    Geo g;
+    int rc = make_geo(shape, nullptr, &g, false);
+    if (rc) return rc;
+    if (!bytes) return fail(QWFN_EINVAL, "bytes is NULL");
+    WinPlan p{n_seq, n_rows, max_q, max_seq_len, window, sink_tokens, dtype, false};
+    if ((rc = check_window("window_workspace", g, p))) return rc;
+    WinPlan d = p;                                    // the decode call of the same sequences
+    d.n_rows = d.n_seq;
+    d.max_q = 1;
+    p.prefill = true;
+    *bytes = std::max(window_ws_bytes(g, d), max_q == 1 && n_rows <= n_seq ? (size_t)0 : window_ws_bytes(g, p));
+    return ok();
+}
+
+static int window_attn(const char *what, const qwfn_qsa_shape *shape, const qwfn_kv_view *view, const WinPlan &p,
+                       const WinArg &wa, void *ws, size_t ws_bytes, void *stream) {
+    Geo g;
+    int rc = make_geo(shape, view, &g);
+    if (rc) return rc;
+    if ((rc = check_window(what, g, p))) return rc;
+    if (p.n_seq > view->n_seq) return fail(QWFN_EINVAL, "%s: n_seq %d > view n_seq %d", what, p.n_seq, view->n_seq);
+    if ((int64_t)p.max_seq_len > (int64_t)g.pps * g.pt)
+        return fail(QWFN_ERANGE, "%s: context exhausted: max_seq_len %d > capacity %lld", what, p.max_seq_len,
+                    (long long)g.pps * g.pt);
+    if (!wa.q || !wa.out || !wa.seq_len || (p.prefill && !wa.q_start))
+        return fail(QWFN_EINVAL, "%s: NULL q, out, seq_len or q_start", what);
+    if (!aligned(wa.q, 16) || !aligned(wa.out, 16) || !aligned(wa.seq_len, 4) || !aligned(wa.q_start, 4))
+        return fail(QWFN_EINVAL, "%s: q and out must be 16-byte aligned, seq_len and q_start 4-byte", what);
+    const size_t bytes = (size_t)p.n_rows * g.H * g.hd * dtype_size(p.dtype);
+    if ((uintptr_t)wa.q < (uintptr_t)wa.out + bytes && (uintptr_t)wa.out < (uintptr_t)wa.q + bytes)
+        return fail(QWFN_EINVAL, "%s: q and out overlap", what);
+    if (!ws || !aligned(ws, 256)) return fail(QWFN_EINVAL, "%s: workspace NULL or not 256-byte aligned", what);
+    const size_t need = window_ws_bytes(g, p);
+    if (ws_bytes < need) return fail(QWFN_ERANGE, "%s: workspace of %zu bytes < %zu needed", what, ws_bytes, need);
+    const hipError_t e = launch_window(g, *view, wa, p, ws, (hipStream_t)stream);
+    return e == hipSuccess ? ok() : hip_fail(e, what);
+}
+
+int qwfn_window_attn_decode(const qwfn_qsa_shape *shape, const qwfn_kv_view *view, const void *q, int32_t dtype,
+                            const int32_t *seq_len, int32_t n_seq, int32_t max_seq_len, int32_t window,
+                            int32_t sink_tokens, void *out, void *ws, size_t ws_bytes, void *stream) {
+    return window_attn("window_attn_decode", shape, view,
+                       WinPlan{n_seq, n_seq, 1, max_seq_len, window, sink_tokens, dtype, false},
+                       WinArg{q, out, nullptr, seq_len, dtype, n_seq, n_seq, 1, max_seq_len, window, sink_tokens}, ws,
+                       ws_bytes, stream);
+}
+
+int qwfn_window_attn_prefill(const qwfn_qsa_shape *shape, const qwfn_kv_view *view, const void *q, int32_t dtype,
+                             const int32_t *q_start, const int32_t *seq_len, int32_t n_seq, int32_t n_rows,
+                             int32_t max_q, int32_t max_seq_len, int32_t window, int32_t sink_tokens, void *out,
+                             void *ws, size_t ws_bytes, void *stream) {
+    return window_attn("window_attn_prefill", shape, view,
+                       WinPlan{n_seq, n_rows, max_q, max_seq_len, window, sink_tokens, dtype, true},
+                       WinArg{q, out, q_start, seq_len, dtype, n_seq, n_rows, max_q, max_seq_len, window, sink_tokens},
+                       ws, ws_bytes, stream);
+}
+
 }  // extern "C"

@@ -173,6 +173,39 @@ __device__ __forceinline__ uint32_t quant_q4(const float x[4], int e, uint16_t *
     return (q[0] | q[2] << 4) | ((q[1] | q[3] << 4) << 8);
 }
 
+// One lane's 4 values of one 32-value block of a head row, quantized (q8_0,
+// q4_0) or converted (F16) and stored at (page, row) with the block's scale:
+// lane e4 of the block's 8 (which must be active together: the quantizers' DPP
+// and shuffles span them) takes the values get2 / get4 give for an offset in
+// the head row.
+template <class Get2, class Get4>
+__device__ __forceinline__ void store_block_lane(const Geo &g, uint8_t *page, bool is_v, int gh, int row, int j,
+                                                 int e4, Get2 get2, Get4 get4) {
+    float x[4];
+    if (g.kt == QWFN_KV_Q4_0) {
+        float a[2], b[2];
+        get2(32 * j + 2 * e4, a);
+        get2(32 * j + 16 + 2 * e4, b);
+        x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
+        uint16_t dh;
+        const uint32_t qs = quant_q4(x, e4, &dh);
+        *reinterpret_cast<uint16_t *>(page + chunk_off(g, gh, row, j) + 2 * e4) = (uint16_t)qs;
+        if (e4 == 0) *reinterpret_cast<uint16_t *>(page + scale_off(g, gh, row, j)) = dh;
+    } else if (g.kt == QWFN_KV_F16) {
+        get4(32 * j + 4 * e4, x);
+        const uint32_t lo = (uint32_t)f2h(x[0]) | (uint32_t)f2h(x[1]) << 16;
+        const uint32_t hi = (uint32_t)f2h(x[2]) | (uint32_t)f2h(x[3]) << 16;
+        const int d = 32 * j + 4 * e4;
+        *reinterpret_cast<uint2 *>(page + chunk_off(g, gh, row, d / 8) + (d % 8) * 2) = make_uint2(lo, hi);
+    } else {
+        get4(32 * j + 4 * e4, x);
+        uint16_t dh;
+        const uint32_t pk = quant4(x, g.variant, &dh, nullptr);
+        store_q4(g, page, is_v, gh, row, 32 * j + 4 * e4, pk);
+        if (e4 == 0) *reinterpret_cast<uint16_t *>(page + scale_off(g, gh, row, j)) = dh;
+    }
+}
+
 // One lane of a K/V row append (k_append, and the decode step's append in
 // k_idx_append_pool): lane i quantizes (q8_0, q4_0) or converts (F16) 4 values
 // of one 32-value block and stores them with the block's scale.  Blocks
@@ -199,32 +232,11 @@ __device__ __forceinline__ void append_lane(const Geo &g, const qwfn_kv_view &v,
     const int32_t pp = phys_page(g, v.page_table, seq, t);
     if (pp < 0) { if (report) set_status(v.status, QWFN_STATUS_PAGE_RANGE); return; }
     const void *src = which ? vsrc : ksrc;
-    const int64_t base = ((int64_t)r * g.Hkv + gh) * g.hd + 32 * j;
+    const int64_t base = ((int64_t)r * g.Hkv + gh) * g.hd;
     uint8_t *page = (uint8_t *)(which ? v.v_pages : v.k_pages) + (int64_t)pp * g.page_bytes;
     const int row = t % g.pt;
-    float x[4];
-    if (g.kt == QWFN_KV_Q4_0) {
-        float a[2], b[2];
-        load2(src, f16, base + 2 * e4, a);
-        load2(src, f16, base + 16 + 2 * e4, b);
-        x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
-        uint16_t dh;
-        const uint32_t qs = quant_q4(x, e4, &dh);
-        *reinterpret_cast<uint16_t *>(page + chunk_off(g, gh, row, j) + 2 * e4) = (uint16_t)qs;
-        if (e4 == 0) *reinterpret_cast<uint16_t *>(page + scale_off(g, gh, row, j)) = dh;
-    } else if (g.kt == QWFN_KV_F16) {
-        load4(src, f16, base + 4 * e4, x);
-        const uint32_t lo = (uint32_t)f2h(x[0]) | (uint32_t)f2h(x[1]) << 16;
-        const uint32_t hi = (uint32_t)f2h(x[2]) | (uint32_t)f2h(x[3]) << 16;
-        const int d = 32 * j + 4 * e4;
-        *reinterpret_cast<uint2 *>(page + chunk_off(g, gh, row, d / 8) + (d % 8) * 2) = make_uint2(lo, hi);
-    } else {
-        load4(src, f16, base + 4 * e4, x);
-        uint16_t dh;
-        const uint32_t pk = quant4(x, g.variant, &dh, nullptr);
-        store_q4(g, page, which, gh, row, 32 * j + 4 * e4, pk);
-        if (e4 == 0) *reinterpret_cast<uint16_t *>(page + scale_off(g, gh, row, j)) = dh;
-    }
+    store_block_lane(g, page, which, gh, row, j, e4, [&](int d, float *x) { load2(src, f16, base + d, x); },
+                     [&](int d, float *x) { load4(src, f16, base + d, x); });
 }
 
 // One dequantized value straight from global memory (gather path): q8_0

@@ -382,4 +382,43 @@ hipError_t launch_gather(const Geo &g, const qwfn_kv_view &v, const int32_t *seq
                          int32_t max_sel, float *k_out, float *v_out, int32_t *cells,
                          hipStream_t st);
 
+
+// ---- rotary positions (qsa_rope.hip) ----
+constexpr int kRopeMaxDim = 512;          // values of a head row
+struct RopeArg {
+    const double *turns;                  // [rd/2] turns a position of each pair
+    int32_t rd, interleaved, inverse;
+    double mscale, eps;
+};
+// Head rows in memory: value d of row r's head h at r * row_stride + h * head_stride + d.
+struct RowsArg {
+    void *data;
+    int32_t dtype;                        // QWFN_SRC_*
+    int64_t row_stride, head_stride;
+};
+hipError_t launch_rope_rows(const RopeArg &rp, const RowsArg &src, const float *norm, const int32_t *pos,
+                            int32_t n_rows, int32_t heads, int32_t hd, const RowsArg &dst, hipStream_t st);
+// K (turned) and V into the cache at (seq_ids[r] or 0, pos[r]); q.data != NULL: q turned into q_out too
+hipError_t launch_rope_append(const Geo &g, const qwfn_kv_view &v, const RopeArg &rp, const RowsArg &q,
+                              const RowsArg &k, const RowsArg &vv, const float *q_norm, const float *k_norm,
+                              const int32_t *seq_ids, const int32_t *pos, int32_t n_rows, const RowsArg &q_out,
+                              hipStream_t st);
+
+// ---- sliding-window attention (qsa_window.hip) ----
+// What the host knows of a call, and what its workspace is sized for.
+struct WinPlan {
+    int32_t n_seq, n_rows, max_q, max_seq_len, window, sinks, dtype;
+    bool prefill;
+};
+struct WinArg {
+    const void *q;                        // [n_rows][H][hd]
+    void *out;
+    const int32_t *q_start;               // [n_seq + 1] rows of each sequence; NULL: row s is sequence s's
+    const int32_t *seq_len;               // [n_seq]
+    int32_t dtype, n_seq, n_rows, max_q, max_seq_len, window, sinks;
+};
+size_t window_ws_bytes(const Geo &g, const WinPlan &p);
+hipError_t launch_window(const Geo &g, const qwfn_kv_view &v, const WinArg &wa, const WinPlan &p, void *ws,
+                         hipStream_t st);
+
 }  // namespace qwfn_qsa

@@ -15,13 +15,14 @@ Every function takes device tensors and enqueues on the current HIP stream
 from __future__ import annotations
 
 import ctypes as C
+import math
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence
 
 import torch
 
 from . import _lib
-from ._lib import IdxShape, IdxView, KvView, QsaShape, call
+from ._lib import IdxShape, IdxView, KvView, QsaShape, RopeStruct, RowsStruct, call
 
 __all__ = [
     "QsaConfig", "KvCache", "KvState", "Workspace",
@@ -30,6 +31,7 @@ __all__ = [
     "export_rows_q8_0", "import_rows_q8_0", "read_status", "time_next_call",
     "IdxConfig", "IdxCache", "idx_append_pool", "idx_pool_rebuild", "idx_select", "idx_sparse_attn_prefill",
     "checkpoint_config",
+    "RopeConfig", "Rope", "rope_rows", "append_rope", "window_attn_decode", "window_attn_prefill",
 ]
 
 
@@ -103,6 +105,14 @@ class QsaConfig:
         call("qwfn_qsa_prefill_workspace_bytes", C.byref(s), max_seq_len, q_batch, C.byref(out))
         return out.value
 
+    def window_workspace_bytes(self, n_seq: int, n_rows: int, max_q: int, max_seq_len: int, window: int,
+                               sink_tokens: int = 0, dtype: torch.dtype = torch.float32) -> int:
+        out = C.c_size_t()
+        s = self.shape()
+        call("qwfn_window_workspace_bytes", C.byref(s), n_seq, n_rows, max_q, max_seq_len, window, sink_tokens,
+             _dtype(dtype, "dtype"), C.byref(out))
+        return out.value
+
     def dense(self) -> "QsaConfig":
         """The same layer with the selection switched off (the reference's
         ``qsa == nullptr`` dense path, src/qwfn_graph.cpp:85-89)."""
@@ -124,6 +134,16 @@ def _stream(stream) -> int:
     if isinstance(stream, torch.cuda.Stream):
         return stream.cuda_stream
     return int(stream)
+
+
+_DTYPES = {torch.float32: _lib.SRC_F32, torch.float16: _lib.SRC_F16, torch.bfloat16: _lib.SRC_BF16}
+
+
+def _dtype(t: torch.dtype, name: str) -> int:
+    got = _DTYPES.get(t)
+    if got is None:
+        raise TypeError(f"{name} must be float32, float16 or bfloat16, got {t}")
+    return got
 
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: Optional[int] = None) -> None:
@@ -277,6 +297,16 @@ class Workspace:
                     stream=None) -> "Workspace":
         """Workspace for :func:`sparse_attn_prefill` taking q_batch queries per launch pair."""
         return cls(cfg, 1, max_seq_len, device, stream, nbytes=cfg.prefill_workspace_bytes(max_seq_len, q_batch))
+
+    @classmethod
+    def for_window(cls, cfg: QsaConfig, n_seq: int, max_seq_len: int, window: int, sink_tokens: int = 0,
+                   n_rows: Optional[int] = None, max_q: int = 1, dtype: torch.dtype = torch.float32, device="cuda",
+                   stream=None) -> "Workspace":
+        """Workspace for :func:`window_attn_decode` over n_seq sequences and, with n_rows (and max_q of one
+        sequence), for :func:`window_attn_prefill` of that many query rows of ``dtype``."""
+        return cls(cfg, n_seq, max_seq_len, device, stream,
+                   nbytes=cfg.window_workspace_bytes(n_seq, n_seq if n_rows is None else n_rows, max_q, max_seq_len,
+                                                     window, sink_tokens, dtype))
 
     def ptr(self) -> int:
         return self.buf.data_ptr()
@@ -808,4 +838,237 @@ def idx_sparse_attn_prefill(ic: IdxCache, q: torch.Tensor, q_idx: torch.Tensor, 
     call("qwfn_idx_sparse_attn_prefill", C.byref(ic.kv.c_shape()), C.byref(cache.view()), C.byref(ic.c_shape()),
          C.byref(ic.view()), q.data_ptr(), q_idx.data_ptr(), _ptr(k_new), _ptr(v_new), _ptr(k_raw), src, seq,
          pos0, n_q, out.data_ptr(), _ptr(sel), _ptr(n_sel), max_sel, ws.ptr(), ws.nbytes, _stream(stream))
+    return out
+
+
+# ---- rotary positions -------------------------------------------------------
+
+@dataclass(frozen=True)
+class RopeConfig:
+    """A rotation of the first ``rope_dim`` values of a head row: frequencies
+    base^(-2i / rope_dim), pairs (i, i + rope_dim / 2) ("half", the reference's
+    IMROPE for text, src/qwfn_graph.cpp:410-429) or (2i, 2i + 1)
+    ("interleaved").  Scaled for contexts past the ``trained_tokens``:
+
+    * "linear": every frequency over ``factor``;
+    * "yarn" (Peng et al., "YaRN", 2023): pairs of more than ``beta_fast`` turns
+      over the trained length keep theirs, pairs of fewer than ``beta_slow``
+      have it over ``factor``, a ramp between; ``mscale`` (None: 0.1 ln(factor)
+      + 1) multiplies cos and sin.
+
+    ``norm_eps`` belongs to the RMSNorm of the calls that are given its weights."""
+    rope_dim: int = 128
+    base: float = 10000000.0
+    layout: str = "half"
+    scaling: str = "none"
+    factor: float = 1.0
+    trained_tokens: int = 32768
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    mscale: Optional[float] = None
+    norm_eps: float = 1e-6
+
+    def __post_init__(self):
+        if self.rope_dim < 2 or self.rope_dim % 2:
+            raise ValueError(f"rope_dim {self.rope_dim} must be an even number >= 2")
+        if self.layout not in ("half", "interleaved"):
+            raise ValueError(f"layout {self.layout!r} is not 'half' or 'interleaved'")
+        if self.scaling not in ("none", "linear", "yarn"):
+            raise ValueError(f"scaling {self.scaling!r} is not 'none', 'linear' or 'yarn'")
+        if not self.base > 1.0 or not self.factor > 0.0 or self.trained_tokens < 1:
+            raise ValueError("base must be > 1, factor > 0 and trained_tokens >= 1")
+
+    def frequencies(self) -> List[float]:
+        """Radians a position of each pair."""
+        d = self.rope_dim
+        freq = [self.base ** (-2.0 * i / d) for i in range(d // 2)]
+        if self.scaling == "none":
+            return freq
+        if self.scaling == "linear":
+            return [f / self.factor for f in freq]
+
+        def pair_of(turns: float) -> float:          # the pair that makes so many turns over the trained length
+            return d * math.log(self.trained_tokens / (turns * 2.0 * math.pi)) / (2.0 * math.log(self.base))
+
+        low = max(math.floor(pair_of(self.beta_fast)), 0)
+        high = min(math.ceil(pair_of(self.beta_slow)), d - 1)
+        ramp = [min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(d // 2)]
+        return [f / self.factor * r + f * (1.0 - r) for f, r in zip(freq, ramp)]
+
+    def scale(self) -> float:
+        """The factor on cos and sin."""
+        if self.mscale is not None:
+            return self.mscale
+        return 0.1 * math.log(self.factor) + 1.0 if self.scaling == "yarn" and self.factor > 1.0 else 1.0
+
+
+class Rope:
+    """A :class:`RopeConfig`'s table on a device (``turns``: turns a position of
+    each pair, float64) and its C struct.  ``turns`` given: frequencies of the
+    caller's own, over 2 pi."""
+
+    def __init__(self, cfg: RopeConfig, device="cuda", turns: Optional[torch.Tensor] = None):
+        if turns is None:
+            turns = torch.tensor([f / (2.0 * math.pi) for f in cfg.frequencies()], dtype=torch.float64)
+        if turns.numel() != cfg.rope_dim // 2:
+            raise ValueError(f"turns has {turns.numel()} values, expected {cfg.rope_dim // 2}")
+        self.cfg = cfg
+        self.turns = turns.to(device=device, dtype=torch.float64).contiguous()
+        self._c = RopeStruct(cfg.rope_dim, _lib.ROPE_HALF if cfg.layout == "half" else _lib.ROPE_INTERLEAVED,
+                             self.turns.data_ptr(), cfg.scale(), cfg.norm_eps)
+
+    def c_struct(self) -> RopeStruct:
+        return self._c
+
+
+def _rows(t: torch.Tensor, name: str, n_rows: int, n_heads: int, head_dim: int, device: torch.device) -> RowsStruct:
+    """Head rows [n_rows, n_heads, head_dim] with any row and head stride."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    dtype = _dtype(t.dtype, name)
+    if t.device != device or device.type != "cuda":
+        raise ValueError(f"{name} must be on the device of the other tensors, {device}; it is on {t.device}")
+    if tuple(t.shape) != (n_rows, n_heads, head_dim):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {(n_rows, n_heads, head_dim)}")
+    rs, hs, one = t.stride()
+    if one != 1 and head_dim > 1:
+        raise ValueError(f"{name}: the values of a head row must be contiguous")
+    return RowsStruct(t.data_ptr(), dtype, rs, hs)
+
+
+def _beside(device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} must be on {device}, it is on {t.device}")
+
+
+def _call_on(device: torch.device, stream, name: str, *args) -> None:
+    """An entry point on the tensors' device, whichever is the current one."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, _stream(stream))
+        return
+    with torch.cuda.device(device):
+        call(name, *args, _stream(stream))
+
+
+def rope_rows(rope: Rope, x: torch.Tensor, pos: torch.Tensor, norm: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None, inverse: bool = False, stream=None) -> torch.Tensor:
+    """Head rows x [n_rows, n_heads, head_dim] (float32, float16 or bfloat16,
+    any row and head stride), normed when ``norm`` (float32 [head_dim]) is
+    given, turned by their positions ``pos`` (int32 [n_rows]) into ``out`` (of
+    any of the three types; x itself for in place, default a new tensor of x's
+    type): the norm and rotation of the layer's queries and of the checkpoint
+    indexer's q_idx (src/qwfn_graph.cpp:480-484).  ``inverse`` turns the other
+    way, which is also the gradient of rows that are not normed."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 3:
+        raise ValueError("x must be a tensor [n_rows, n_heads, head_dim]")
+    n, heads, hd = x.shape
+    dev = x.device
+    if out is None:
+        out = torch.empty((n, heads, hd), dtype=x.dtype, device=dev)
+    if n == 0:                                       # no rows: nothing to launch
+        return out
+    src, dst = _rows(x, "x", n, heads, hd, dev), _rows(out, "out", n, heads, hd, dev)
+    _need(pos, "pos", torch.int32, n)
+    if norm is not None:
+        _need(norm, "norm", torch.float32, hd)
+    _beside(dev, pos=pos, norm=norm, turns=rope.turns)
+    _call_on(dev, stream, "qwfn_rope_rows", C.byref(rope.c_struct()), C.byref(src), _ptr(norm), pos.data_ptr(), n,
+             heads, hd, 1 if inverse else 0, C.byref(dst))
+    return out
+
+
+def append_rope(cache: KvCache, rope: Rope, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor,
+                seq_ids: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
+                q: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None,
+                q_out: Optional[torch.Tensor] = None, stream=None) -> Optional[torch.Tensor]:
+    """:func:`append_q8_0` with the rotation on the way: K rows k [n_rows,
+    n_head_kv, head_dim], normed when ``k_norm`` (float32 [head_dim]) is given
+    and turned at ``pos``, and V rows v as they are (float32, float16 or
+    bfloat16, any row and head stride) are written at positions ``pos`` (int32)
+    of ``seq_ids`` (default 0).  With the rows' queries q [n_rows, n_head,
+    head_dim], those are normed (``q_norm``) and turned in the same launch into
+    ``q_out`` (default float32), which is returned."""
+    cfg = cache.cfg
+    n, dev = pos.numel(), cache.k_pages.device
+    if q is None and (q_norm is not None or q_out is not None):
+        raise ValueError("q_norm and q_out come with q")
+    if q is not None and q_out is None:
+        q_out = torch.empty((n, cfg.n_head, cfg.head_dim), dtype=torch.float32, device=dev)
+    if n == 0:
+        return q_out
+    kr, vr = (_rows(t, m, n, cfg.n_head_kv, cfg.head_dim, dev) for t, m in ((k, "k"), (v, "v")))
+    qr = qo = None
+    if q is not None:
+        qr, qo = (_rows(t, m, n, cfg.n_head, cfg.head_dim, dev) for t, m in ((q, "q"), (q_out, "q_out")))
+    _need(pos, "pos", torch.int32, n)
+    if seq_ids is not None:
+        _need(seq_ids, "seq_ids", torch.int32, n)
+    for t, m in ((k_norm, "k_norm"), (q_norm, "q_norm")):
+        if t is not None:
+            _need(t, m, torch.float32, cfg.head_dim)
+    _beside(dev, pos=pos, seq_ids=seq_ids, k_norm=k_norm, q_norm=q_norm, turns=rope.turns)
+    _call_on(dev, stream, "qwfn_kv_append_rope", C.byref(cache.c_shape()), C.byref(cache.view()),
+             C.byref(rope.c_struct()), C.byref(kr), C.byref(vr), _ptr(k_norm), _ptr(seq_ids), pos.data_ptr(), n,
+             None if qr is None else C.byref(qr), _ptr(q_norm), None if qo is None else C.byref(qo))
+    return q_out
+
+
+# ---- sliding-window attention ------------------------------------------------
+
+def _window_rows(cache: KvCache, q: torch.Tensor, n_rows: Optional[int], out: Optional[torch.Tensor], ws: Workspace):
+    cfg, dev = cache.cfg, cache.k_pages.device
+    if not isinstance(q, torch.Tensor):
+        raise TypeError("q must be a torch.Tensor")
+    width = cfg.n_head * cfg.head_dim
+    if n_rows is None:
+        n_rows = q.numel() // width
+    dtype = _dtype(q.dtype, "q")
+    _need(q, "q", q.dtype, n_rows * width)
+    if out is None:
+        out = torch.empty((n_rows, cfg.n_head, cfg.head_dim), dtype=q.dtype, device=dev)
+    _need(out, "out", q.dtype, n_rows * width)
+    _beside(dev, q=q, out=out, ws=ws.buf)
+    return dtype, n_rows, out, dev
+
+
+def window_attn_decode(cache: KvCache, q: torch.Tensor, seq_len: torch.Tensor, max_seq_len: int, window: int,
+                       ws: Workspace, sink_tokens: int = 0, out: Optional[torch.Tensor] = None,
+                       stream=None) -> torch.Tensor:
+    """Attention of one query a sequence (q [n_seq, n_head, head_dim] float32,
+    float16 or bfloat16, at position seq_len - 1) over the last ``window``
+    cells and the first ``sink_tokens`` ones, exact to the token: the dense
+    attention of the reference's decode (src/qwfn_graph.cpp:497-542) with a
+    sliding window.  ``out`` has q's type.  A sequence of length 0 gets zeros;
+    pages that no visible cell is in may be given back."""
+    n_seq = seq_len.numel()
+    _need(seq_len, "seq_len", torch.int32)
+    dtype, _, out, dev = _window_rows(cache, q, n_seq, out, ws)
+    _beside(dev, seq_len=seq_len)
+    if n_seq == 0:
+        return out
+    _call_on(dev, stream, "qwfn_window_attn_decode", C.byref(cache.c_shape()), C.byref(cache.view()), q.data_ptr(),
+             dtype, seq_len.data_ptr(), n_seq, max_seq_len, window, sink_tokens, out.data_ptr(), ws.ptr(), ws.nbytes)
+    return out
+
+
+def window_attn_prefill(cache: KvCache, q: torch.Tensor, q_start: torch.Tensor, seq_len: torch.Tensor, max_q: int,
+                        max_seq_len: int, window: int, ws: Workspace, sink_tokens: int = 0,
+                        out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """:func:`window_attn_decode` for several queries a sequence: rows
+    q_start[s] .. q_start[s + 1] (int32 [n_seq + 1], device) of q [n_rows,
+    n_head, head_dim] are the last positions of sequence s, whose length with
+    them is seq_len[s]; their K and V are in the cache already
+    (:func:`append_rope`).  ``max_q`` bounds one sequence's rows.  Rows outside
+    every sequence are left as they were."""
+    n_seq = seq_len.numel()
+    _need(seq_len, "seq_len", torch.int32)
+    _need(q_start, "q_start", torch.int32, n_seq + 1)
+    dtype, n_rows, out, dev = _window_rows(cache, q, None, out, ws)
+    _beside(dev, seq_len=seq_len, q_start=q_start)
+    if n_seq == 0 or n_rows == 0:
+        return out
+    _call_on(dev, stream, "qwfn_window_attn_prefill", C.byref(cache.c_shape()), C.byref(cache.view()), q.data_ptr(),
+             dtype, q_start.data_ptr(), seq_len.data_ptr(), n_seq, n_rows, max_q, max_seq_len, window, sink_tokens,
+             out.data_ptr(), ws.ptr(), ws.nbytes)
     return out
