@@ -517,7 +517,8 @@ int qwfn_kv_append_rope(const qwfn_qsa_shape *shape, const qwfn_kv_view *view, c
  * attended.  A cell that a query does not see does not change its result,
  * whatever it holds; a NaN or infinity that it sees makes its output (from V:
  * that value of it) NaN or infinite.
- * n_head / n_head_kv is at most 16 (QWFN_ENOTSUP).                             */
+ * Heads of 64, 128 or 256 values, up to 8 query heads a KV head, or 16 of 256
+ * (else QWFN_ENOTSUP).                                                         */
 
 /* Workspace of the two calls for up to n_seq sequences, n_rows query rows of
  * dtype, max_q of one sequence and max_seq_len tokens (n_rows = n_seq, max_q =

@@ -1266,7 +1266,8 @@ int qwfn_kv_append_rope(const qwfn_qsa_shape *shape, const qwfn_kv_view *view, c
 static int check_window(const char *what, const Geo &g, const WinPlan &p) {
     int rc = check_dtype(what, p.dtype);
     if (rc) return rc;
-    if (g.G > 16) return fail(QWFN_ENOTSUP, "%s: %d query heads a KV head, at most 16", what, g.G);
+    if (!win_shape(g.hd, g.G))
+        return fail(QWFN_ENOTSUP, "%s: no kernel for head_dim %d with %d query heads a KV head", what, g.hd, g.G);
     if (p.window < 1) return fail(QWFN_EINVAL, "%s: window %d < 1", what, p.window);
     if (p.sinks < 0) return fail(QWFN_EINVAL, "%s: sink_tokens %d < 0", what, p.sinks);
     if (p.n_seq < 1 || p.n_rows < 1 || p.max_q < 1 || p.max_seq_len < 1)

@@ -417,6 +417,7 @@ struct WinArg {
     const int32_t *seq_len;               // [n_seq]
     int32_t dtype, n_seq, n_rows, max_q, max_seq_len, window, sinks;
 };
+bool win_shape(int32_t hd, int32_t G);    // an instantiation exists
 size_t window_ws_bytes(const Geo &g, const WinPlan &p);
 hipError_t launch_window(const Geo &g, const qwfn_kv_view &v, const WinArg &wa, const WinPlan &p, void *ws,
                          hipStream_t st);

@@ -1,0 +1,89 @@
+// qsa_window.h -- what the sliding-window kernels share: a sequence's list of
+// 64-cell tiles, rows of the three element types, the parts' merge.
+#pragma once
+
+#include <algorithm>
+
+#include "qsa_device.h"
+
+namespace qwfn_qsa {
+
+inline size_t win_align(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// The 64-cell tiles that the last n_q queries of a sequence of length len see: the
+// first tokens' tiles 0 .. ns - 1, then the window's from tile w0 (no tile twice).
+struct WinTiles {
+    int n, ns, w0, window, sinks;
+    __host__ __device__ __forceinline__ int cell(int i) const { return (i < ns ? i : w0 + i - ns) * 64; }
+    // the cells the query at position len - 1 sees
+    __device__ __forceinline__ bool seen(int t, int len) const { return t < len && (t >= len - window || t < sinks); }
+    __device__ __forceinline__ bool whole(int i, int len) const {
+        const int t = cell(i);
+        return t + 64 <= len && (t >= len - window || t + 64 <= sinks);
+    }
+};
+__host__ __device__ __forceinline__ WinTiles win_tiles(int len, int n_q, int window, int sinks) {
+    WinTiles t;
+    t.window = window;
+    t.sinks = sinks;
+    t.n = t.ns = t.w0 = 0;
+    if (len <= 0) return t;
+    const int64_t lo = (int64_t)len - n_q - window + 1;
+    const int first = lo > 0 ? (int)lo : 0;
+    const int s = sinks < first ? sinks : first;        // first tokens before the window
+    t.ns = (s + 63) / 64;
+    t.w0 = first / 64 > t.ns ? first / 64 : t.ns;
+    t.n = t.ns + (len + 63) / 64 - t.w0;
+    return t;
+}
+// The most tiles such a list has within a plan's bounds.
+inline int win_most_tiles(const WinPlan &p) {
+    const int64_t all = ((int64_t)p.max_seq_len + 63) / 64;
+    const int64_t win = ((int64_t)p.window + p.max_q - 1 + 126) / 64, sink = ((int64_t)p.sinks + 63) / 64;
+    return (int)std::min<int64_t>(all, win + sink);
+}
+
+__device__ __forceinline__ float bf16_f(uint32_t h) { return __uint_as_float(h << 16); }
+
+// Eight values of a row at a 16-byte (fp32: 32-byte run's) boundary.
+__device__ __forceinline__ void load8(const void *p, int dtype, int64_t i, float *x) {
+    if (dtype == QWFN_SRC_F32) {
+        const f4v a = *reinterpret_cast<const f4v *>((const float *)p + i), b = *reinterpret_cast<const f4v *>((const float *)p + i + 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { x[k] = a[k]; x[4 + k] = b[k]; }
+    } else {
+        const u4v w = *reinterpret_cast<const u4v *>((const uint16_t *)p + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            x[2 * k] = dtype == QWFN_SRC_F16 ? h2f((uint16_t)w[k]) : bf16_f(w[k] & 0xFFFFu);
+            x[2 * k + 1] = dtype == QWFN_SRC_F16 ? h2f((uint16_t)(w[k] >> 16)) : bf16_f(w[k] >> 16);
+        }
+    }
+}
+// Four values of a row.
+__device__ __forceinline__ void store4(void *p, int dtype, int64_t i, f4v y) {
+    if (dtype == QWFN_SRC_F32) {
+        *reinterpret_cast<f4v *>((float *)p + i) = y;
+    } else if (dtype == QWFN_SRC_F16) {
+        typedef _Float16 h4v __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<h4v *>((uint16_t *)p + i) = __builtin_convertvector(y, h4v);
+    } else {
+        typedef __bf16 b4v __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<b4v *>((uint16_t *)p + i) = __builtin_convertvector(y, b4v);
+    }
+}
+
+// The exponent e that brings a row's largest magnitude m to [2^k, 2^(k + 1)): x 2^e.  A
+// zero row and one that is not finite stay as they are.  Bounded so that 2^e and 2^-e
+// are normal numbers.
+__device__ __forceinline__ int pow2_to(float m, int k) {
+    const int b = (int)(__float_as_uint(m) >> 23);      // m >= 0
+    return b == 0 || b == 255 ? 0 : min(max(k + 127 - b, -100), 100);
+}
+
+// Decode (qsa_window_dec.hip)
+int win_dec_parts(const Geo &g, const WinPlan &p);
+size_t win_dec_ws_bytes(const Geo &g, const WinPlan &p);
+hipError_t launch_win_dec(const Geo &g, const qwfn_kv_view &v, const WinArg &wa, const WinPlan &p, void *ws, hipStream_t st);
+
+}  // namespace qwfn_qsa

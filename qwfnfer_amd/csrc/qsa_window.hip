@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include "qsa_append.h"
+#include "qsa_window.h"
 
 namespace qwfn_qsa {
 
@@ -89,10 +90,11 @@ k_window(Geo g, qwfn_kv_view v, WinArg wa) {
     if (tid < g.hd) put_io_value(wa.out, wa.dtype, o + tid, l != 0.0f ? acc / l : 0.0f);
 }
 
-size_t window_ws_bytes(const Geo &g, const WinPlan &p) { return 256; }
+size_t window_ws_bytes(const Geo &g, const WinPlan &p) { return p.prefill ? 256 : win_dec_ws_bytes(g, p); }
 
 hipError_t launch_window(const Geo &g, const qwfn_kv_view &v, const WinArg &wa, const WinPlan &p, void *ws,
                          hipStream_t st) {
+    if (!p.prefill) return launch_win_dec(g, v, wa, p, ws, st);
     hipLaunchKernelGGL(k_window, dim3((unsigned)p.n_rows, (unsigned)g.H), dim3(256), 0, st, g, v, wa);
     return hipGetLastError();
 }
