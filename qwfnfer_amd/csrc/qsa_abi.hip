@@ -1293,7 +1293,7 @@ int qwfn_window_workspace_bytes(const qwfn_qsa_shape *shape, int32_t n_seq, int3
     d.n_rows = d.n_seq;
     d.max_q = 1;
     p.prefill = true;
-    *bytes = std::max(window_ws_bytes(g, d), max_q == 1 && n_rows <= n_seq ? (size_t)0 : window_ws_bytes(g, p));
+    *bytes = std::max(window_ws_bytes(g, d), window_ws_bytes(g, p));
     return ok();
 }
 

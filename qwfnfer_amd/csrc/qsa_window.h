@@ -86,4 +86,8 @@ int win_dec_parts(const Geo &g, const WinPlan &p);
 size_t win_dec_ws_bytes(const Geo &g, const WinPlan &p);
 hipError_t launch_win_dec(const Geo &g, const qwfn_kv_view &v, const WinArg &wa, const WinPlan &p, void *ws, hipStream_t st);
 
+// The parts of every row of the call (part_o, part_rl: [row][Hkv][parts][G]) into out; rows
+// outside every sequence are left as they were.
+void launch_win_merge(const Geo &g, const WinArg &wa, int parts, const float *part_o, const float2 *part_rl, hipStream_t st);
+
 }  // namespace qwfn_qsa

@@ -1,10 +1,20 @@
 // qsa_window.hip -- attention with a sliding window and a few first tokens that
-// stay visible, over the paged cache (qwfn_window_attn_decode,
-// qwfn_window_attn_prefill).
+// stay visible, over the paged cache (qwfn_window_attn_prefill; the single-token
+// kernels are in qsa_window_dec.hip).
 //
 // Mathematics.  The query at position p of a sequence sees the cells t <= p with
-// t > p - window or t < sinks; o = sum_t e^(q.k_t / sqrt(hd) - m) v_t / sum_t
-// e^(q.k_t / sqrt(hd) - m), m the largest visible logit.
+// t > p - window or t < sinks; o = sum_t 2^(s_t - r) v_t / sum_t 2^(s_t - r), s = q.k
+// log2(e) / sqrt(hd), r a running reference near the largest visible s, one pass
+// over the cells.
+//
+// k_win_stage brings the cells that a call's queries see into matrix-core operands
+// once: each would otherwise be unpacked by every block of queries that sees it (a
+// block of 16 queries a time at 8 heads a KV head, so 256 times for a window of
+// 4,096).  k_win_rows walks a block of rows (query x head of one KV head) over its
+// tiles:
+//   S^T = K Q^T on v_mfma_f32_32x32x16_f16, A = 32 cells, columns = 32 rows;
+//   O^T = V^T P^T, the accumulator layout of S^T being (with V's cells staged in its
+//     order) the operand layout of P^T, so weights never leave their lane.
 #include <hip/hip_runtime.h>
 
 #include "qsa_append.h"
@@ -12,91 +22,524 @@
 
 namespace qwfn_qsa {
 
+typedef float f16v __attribute__((ext_vector_type(16)));
+
 namespace {
 
-__device__ __forceinline__ float io_value(const void *p, int dtype, int64_t i) {
-    if (dtype == QWFN_SRC_F32) return ((const float *)p)[i];
-    const uint16_t h = ((const uint16_t *)p)[i];
-    return dtype == QWFN_SRC_F16 ? h2f(h) : __uint_as_float((uint32_t)h << 16);
+// A staged tile of 64 cells of one KV head, NP planes (fp16, or fp16 hi and lo):
+//   K [plane][hd / 8][64 cells][8 dims]
+//   V [plane][64 / 16][2][hd][8 cells]: cells 16 ks + 4 half + {0 .. 3, 8 .. 11}
+template <int HD, int NP> constexpr int staged_half() { return NP * 64 * HD * 2; }     // bytes of K, or of V
+// What the rows' kernel needs to know of it: values are staged times 2^ke, 2^ve.
+struct TileInfo {
+    int32_t ke, ve;
+    int32_t there;          // the tile's page is in the pool
+    int32_t odd;            // V holds values that are not finite
+};
+
+// A plan's staging area: tiles [n_seq][Hkv][cap], their TileInfo, then the parts.
+struct PfLayout {
+    int cap, parts, blocks;
+    size_t info, part_o, part_rl, total;
+};
+
+constexpr int kExact = 2;   // planes of float32 and float16 rows
+
+// The sequence's queries and length, and whether they can be served.
+struct PfSeq { int start, n_q, len; bool ok; };
+__device__ __forceinline__ PfSeq pf_seq(const WinArg &wa, int s) {
+    PfSeq q;
+    q.start = wa.q_start[s];
+    q.n_q = wa.q_start[s + 1] - q.start;
+    q.len = wa.seq_len[s];
+    if (q.start < 0 || q.n_q < 0 || q.n_q > wa.n_rows - q.start) { q.n_q = 0; q.ok = false; return q; }
+    q.ok = q.len >= 0 && q.len <= wa.max_seq_len && q.n_q <= q.len && q.n_q <= wa.max_q;
+    return q;
 }
-__device__ __forceinline__ void put_io_value(void *p, int dtype, int64_t i, float y) {
-    if (dtype == QWFN_SRC_F32) ((float *)p)[i] = y;
-    else if (dtype == QWFN_SRC_F16) ((uint16_t *)p)[i] = f2h(y);
-    else ((__bf16 *)p)[i] = (__bf16)y;
+
+// e with |x| 2^e < 2^15 for |x| <= m, in steps, so that neighbouring tiles mostly share it
+// (a change costs the rows' kernel a pass over its sums).  fp16's absolute half step 2^-25 is
+// then small against the tile's largest value: one plane, 0 while m is in [2^-4, 2^15), so
+// 2^-21 of m; two planes, multiples of 8, which leave m >= 2^7, so 2^-32.
+template <int NP>
+__device__ __forceinline__ int stage_exp(float m) {
+    const int e = m == 0.0f ? 0 : pow2_to(m, 14);
+    return NP == 2 ? e & ~7 : m >= 0.0625f && m < 32768.0f ? 0 : e;
 }
 
 }  // namespace
 
-// One workgroup a (row, query head): tiles of 64 cells, the running maximum and
-// sum over them, thread d the output's dimension d.
+// grid (tile slots, Hkv, n_seq): slot i of a sequence's list of tiles into its place.
+template <int HD, int KT, bool VD, int NP>
 __global__ void __launch_bounds__(256)
-k_window(Geo g, qwfn_kv_view v, WinArg wa) {
-    __shared__ float part[4][64], p[64], qs[256];
-    const int row = blockIdx.x, h = blockIdx.y, gh = h / g.G, tid = threadIdx.x;
-    int s = row, len, first = 0, n_q = 1;
-    if (wa.q_start) {                       // the last sequence that starts at or before the row
-        int lo = 0, hi = wa.n_seq - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (wa.q_start[mid] <= row) lo = mid; else hi = mid - 1;
-        }
-        s = lo;
-        first = wa.q_start[s];
-        n_q = wa.q_start[s + 1] - first;
-        if (row < first || row >= first + n_q) return;          // behind the last sequence
-    } else {
-        first = row;
-    }
-    len = wa.seq_len[s];
-    const int64_t o = ((int64_t)row * g.H + h) * g.hd;
-    const bool bad = len < 0 || len > wa.max_seq_len || n_q > len + (wa.q_start ? 0 : 1) || n_q > wa.max_q;
-    if (bad || len == 0) {
-        for (int d = tid; d < g.hd; d += 256) put_io_value(wa.out, wa.dtype, o + d, 0.0f);
-        if (bad && tid == 0 && h == 0) set_status(v.status, QWFN_STATUS_LEN_RANGE);
+k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo *info) {
+    constexpr int NB = HD / 32, C8 = HD / 8, kRow = HD + 8;
+    __shared__ float dk[64][NB + 1], dv[64][NB + 1];
+    __shared__ float red[2][4];
+    __shared__ __attribute__((aligned(16))) uint16_t vt[VD ? 1 : 64][VD ? 8 : kRow];
+    const int slot = blockIdx.x, gh = blockIdx.y, s = blockIdx.z, tid = threadIdx.x;
+    const PfSeq q = pf_seq(wa, s);
+    if (!q.ok) {
+        if (slot == 0 && gh == 0 && tid == 0) set_status(v.status, QWFN_STATUS_LEN_RANGE);
         return;
     }
-    const int pos = len - n_q + row - first;
-    for (int d = tid; d < g.hd; d += 256) qs[d] = io_value(wa.q, wa.dtype, o + d) * g.scale_log2;
-    const int lo = pos - wa.window + 1 > 0 ? pos - wa.window + 1 : 0;
-    float m = -INFINITY, l = 0.0f, acc = 0.0f;
-    for (int t0 = 0; t0 <= pos; t0 += 64) {
-        if (t0 >= wa.sinks && t0 + 64 <= lo) { t0 = lo / 64 * 64 - 64; continue; }
-        __syncthreads();
-        const int32_t pp = phys_page(g, v.page_table, s, t0);
-        if (pp < 0) { if (tid == 0) set_status(v.status, QWFN_STATUS_PAGE_RANGE); continue; }
-        const uint8_t *kp = (const uint8_t *)v.k_pages + (int64_t)pp * g.page_bytes;
-        const uint8_t *vp = (const uint8_t *)v.v_pages + (int64_t)pp * g.page_bytes;
-        const int c = tid & 63, w = tid >> 6, n = g.hd / 4;
-        float x = 0.0f;
-        for (int d = w * n; d < (w + 1) * n; ++d) x += qs[d] * member_k(g, kp, gh, (t0 + c) % g.pt, d);
-        part[w][c] = x;
-        __syncthreads();
-        const int t = t0 + c;
-        const bool seen = t <= pos && (t >= lo || t < wa.sinks);
-        x = seen ? (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]) : -INFINITY;
-        const float mt = fmaxf(m, wave_max(x));
-        const float f = m == -INFINITY ? 0.0f : exp2f(m - mt), e = seen ? exp2f(x - mt) : 0.0f;
-        l = l * f + wave_sum(e);
-        m = mt;
-        if (w == 0) p[c] = e;
-        __syncthreads();
-        acc *= f;
-        if (tid < g.hd)
-            for (int i = 0; i < 64; ++i) {
-                const int ti = t0 + i;
-                if (ti <= pos && (ti >= lo || ti < wa.sinks)) acc += p[i] * member_k(g, vp, gh, ti % g.pt, tid, true);
-            }
+    if (q.n_q == 0) return;
+    const WinTiles tl = win_tiles(q.len, q.n_q, wa.window, wa.sinks);
+    if (slot >= tl.n || slot >= cap) return;
+    const int t0 = tl.cell(slot);
+    const int64_t at = ((int64_t)s * g.Hkv + gh) * cap + slot;
+    const int32_t pp = phys_page(g, v.page_table, s, t0);
+    if (pp < 0) {
+        if (tid == 0) {
+            info[at] = TileInfo{0, 0, 0, 0};
+            set_status(v.status, QWFN_STATUS_PAGE_RANGE);
+        }
+        return;
     }
-    if (tid < g.hd) put_io_value(wa.out, wa.dtype, o + tid, l != 0.0f ? acc / l : 0.0f);
+    const int64_t tile = (int64_t)pp * g.page_bytes + (int64_t)(gh * (g.pt / 64) + t0 % g.pt / 64) * g.chunks * 1024;
+    const uint8_t *kq = (const uint8_t *)v.k_pages + tile, *vq = (const uint8_t *)v.v_pages + tile;
+    const int live = q.len - t0;                          // cells of the tile that are written
+    // ---- the scales, and the exponents they ask for ----
+    int ke = 0, ve = 0;
+    if constexpr (KT != QWFN_KV_F16) {
+        const int64_t so = (int64_t)pp * g.page_bytes + g.qbytes + (int64_t)(gh * g.pt + t0 % g.pt) * (NB * 2);
+        const uint16_t *ks = reinterpret_cast<const uint16_t *>((const uint8_t *)v.k_pages + so);
+        const uint16_t *vs = reinterpret_cast<const uint16_t *>((const uint8_t *)v.v_pages + so);
+        float mk = 0.0f, mv = 0.0f;
+        for (int i = tid; i < 64 * NB; i += 256) {
+            const float a = i / NB < live ? h2f(ks[i]) : 0.0f, b = i / NB < live ? h2f(vs[i]) : 0.0f;
+            dk[i / NB][i % NB] = a;
+            dv[i / NB][i % NB] = b;
+            mk = fabsf(a) < INFINITY ? fmaxf(mk, fabsf(a)) : mk;
+            mv = fabsf(b) < INFINITY ? fmaxf(mv, fabsf(b)) : mv;
+        }
+        mk = wave_max(mk);
+        mv = wave_max(mv);
+        if ((tid & 63) == 0) { red[0][tid >> 6] = mk; red[1][tid >> 6] = mv; }
+        __syncthreads();
+        constexpr float kTop = KT == QWFN_KV_Q4_0 ? 8.0f : 128.0f;
+        ke = stage_exp<NP>(kTop * fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3])));
+        ve = stage_exp<NP>(kTop * fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3])));
+    }
+    const float fk = ldexpf(1.0f, ke), fv = ldexpf(1.0f, ve);
+    uint8_t *out = staged + at * (2 * staged_half<HD, NP>());
+    // eight values (8 dims of one cell) of a K-layout tile, times the exponent's power of two
+    auto eight = [&](const uint8_t *tq, const float (*d)[NB + 1], int c8, int cell, float f, float *x) {
+        if constexpr (KT == QWFN_KV_F16) {
+            const u4v w = *reinterpret_cast<const u4v *>(tq + c8 * 1024 + cell * 16);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { x[2 * k] = h2f((uint16_t)w[k]); x[2 * k + 1] = h2f((uint16_t)(w[k] >> 16)); }
+            if (cell >= live)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+        } else {
+            const float dd = d[cell][c8 / 4] * f;
+            if constexpr (KT == QWFN_KV_Q4_0) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(tq + (c8 / 4) * 1024 + cell * 16 + (c8 & 1) * 8);
+                const int sh = c8 & 2 ? 4 : 0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = dd * (float)((int)((k < 4 ? w.x : w.y) >> (8 * (k & 3) + sh) & 15) - 8);
+            } else {
+                const uint2 w = *reinterpret_cast<const uint2 *>(tq + (c8 / 2) * 1024 + cell * 16 + (c8 & 1) * 8);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = dd * (float)(int8_t)((k < 4 ? w.x : w.y) >> (8 * (k & 3)));
+            }
+        }
+    };
+    // plane p of a value: its fp16, or what the fp16 leaves
+    auto plane = [&](float x, int p) {
+        const _Float16 h = (_Float16)x;
+        if (p == 0) return h;
+        return fabsf(x) < INFINITY ? (_Float16)(x - (float)h) : (_Float16)0.0f;
+    };
+    for (int i = tid; i < C8 * 64; i += 256) {
+        float x[8];
+        eight(kq, dk, i >> 6, i & 63, fk, x);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            h8v y;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = plane(x[k], p);
+            *reinterpret_cast<h8v *>(out + (p * C8 * 64 + i) * 16) = y;
+        }
+    }
+    out += staged_half<HD, NP>();
+    int odd = 0;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        if constexpr (!VD) {
+            __syncthreads();
+            for (int i = tid; i < C8 * 64; i += 256) {
+                float x[8];
+                eight(vq, dv, i >> 6, i & 63, fv, x);
+                h8v y;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    y[k] = plane(x[k], p);
+                    odd |= !(fabsf((float)y[k]) < INFINITY);
+                }
+                *reinterpret_cast<h8v *>(&vt[i & 63][(i >> 6) * 8]) = y;
+            }
+            __syncthreads();
+        }
+        for (int i = tid; i < HD * 8; i += 256) {         // i = (ks * 2 + half) * HD + dim
+            const int dim = i % HD, c0 = i / HD / 2 * 16 + (i / HD & 1) * 4;
+            h8v y;
+            if constexpr (VD) {
+                const uint32_t a = *reinterpret_cast<const uint32_t *>(vq + dim * 64 + c0);
+                const uint32_t b = *reinterpret_cast<const uint32_t *>(vq + dim * 64 + c0 + 8);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int cell = c0 + (k < 4 ? k : k + 4);
+                    y[k] = plane(dv[cell][dim / 32] * fv * (float)(int8_t)((k < 4 ? a : b) >> (8 * (k & 3))), p);
+                    odd |= !(fabsf((float)y[k]) < INFINITY);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = __builtin_bit_cast(_Float16, vt[c0 + (k < 4 ? k : k + 4)][dim]);
+            }
+            *reinterpret_cast<h8v *>(out + (p * HD * 8 + i) * 16) = y;
+        }
+    }
+    odd = __syncthreads_or(odd);
+    if (tid == 0) info[at] = TileInfo{ke, ve, 1, odd};
 }
 
-size_t window_ws_bytes(const Geo &g, const WinPlan &p) { return p.prefill ? 256 : win_dec_ws_bytes(g, p); }
+// grid (row blocks * parts, Hkv), four waves of 32 RB rows each; row = query * G + head of
+// the KV head's group.  TC cells a step, double-buffered in LDS.
+template <int HD, int NP, int TC, int RB>
+__global__ void __launch_bounds__(256, HD == 256 || RB == 2 ? 1 : 2)
+k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int parts, const uint8_t *staged, const TileInfo *info, float *part_o,
+           float2 *part_rl) {
+    constexpr int KS = HD / 16, DT = HD / 32, CT = TC / 32, kRows = 128 * RB;
+    constexpr int kHalf = NP * TC * HD * 2, kStep = 2 * kHalf;            // bytes of K (or V), of both
+    constexpr float kOff = NP == 2 ? 13.0f : 6.0f, kSlack = NP == 2 ? 2.0f : 8.0f;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, half = lane >> 5, gh = blockIdx.y, part = blockIdx.x % parts, blk = blockIdx.x / parts;
+    // the block's sequence: blocks of sequence s start at q_start[s] * G / kRows + s
+    int s = 0;
+    for (int hi = wa.n_seq - 1; s < hi;) {
+        const int mid = (s + hi + 1) / 2;
+        if ((int64_t)wa.q_start[mid] * g.G / kRows + mid <= blk) s = mid; else hi = mid - 1;
+    }
+    const PfSeq q = pf_seq(wa, s);
+    const int64_t r0 = (blk - ((int64_t)q.start * g.G / kRows + s)) * kRows;
+    const int64_t total = (int64_t)q.n_q * g.G;
+    if (r0 < 0 || r0 >= total) return;
+    const int base = q.len - q.n_q;                       // position of the sequence's first query
+
+    // ---- the rows' queries ----
+    h8v qf[NP][RB][KS];
+    float c0[RB];
+    int pos[RB];
+    int64_t io[RB];                                       // the row's first value, -1: none
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const int64_t rr = r0 + (w * RB + b) * 32 + n;
+        const int qi = (int)(rr / g.G), h = gh * g.G + (int)(rr % g.G);
+        io[b] = rr < total ? (((int64_t)q.start + qi) * g.H + h) * HD : -1;
+        pos[b] = base + (rr < total ? qi : q.n_q - 1);
+        float x[KS][8], m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            if (io[b] >= 0) {
+                load8(wa.q, wa.dtype, io[b] + 16 * k + 8 * half, x[k]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[k][j] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[k][j]));
+        }
+        m = swap32_op(m, [](float a, float c) { return fmaxf(a, c); });
+        const int e = pow2_to(m, 13);
+        const float f = ldexpf(1.0f, e);
+        c0[b] = ldexpf(g.scale_log2, -e);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = x[k][j] * f;
+                qf[0][b][k][j] = (_Float16)y;
+                if constexpr (NP == 2) qf[NP - 1][b][k][j] = (_Float16)(y - (float)(_Float16)y);
+            }
+    }
+
+    // ---- its tiles: first tokens' tiles before the window, then the window's ----
+    const WinTiles tl = win_tiles(q.ok ? q.len : 0, q.n_q, wa.window, wa.sinks);
+    const int p_lo = base + (int)(r0 / g.G), p_hi = base + (int)((min(r0 + kRows, total) - 1) / g.G);
+    const int wt = max(0, p_lo - wa.window + 1) / 64;
+    const int n1 = min(min(wa.sinks, p_hi + 1) / 64 + (min(wa.sinks, p_hi + 1) % 64 ? 1 : 0), wt);
+    const int nt = q.ok ? (n1 + p_hi / 64 + 1 - wt) * (64 / TC) : 0;
+    const int k0 = (int)((int64_t)nt * part / parts), k1 = (int)((int64_t)nt * (part + 1) / parts);
+    const int64_t first = ((int64_t)s * g.Hkv + gh) * cap;
+    auto cell_of = [&](int k) { const int t = k / (64 / TC); return (t < n1 ? t : wt + t - n1) * 64 + k % (64 / TC) * TC; };
+    auto slot_of = [&](int cell) { const int t = cell / 64; return t < tl.ns ? t : tl.ns + t - tl.w0; };
+    // one step's K and V, 16 bytes a lane, into buffer k & 1
+    auto fetch = [&](int k) {
+        const int cell = cell_of(k);
+        const uint8_t *src = staged + (first + slot_of(cell)) * (int64_t)(2 * staged_half<HD, NP>());
+        const int sub = cell % 64;
+        const uint32_t dst = (uint32_t)(uintptr_t)lds + (k & 1) * kStep;
+#pragma unroll
+        for (int i = 0; i < kHalf / 4096; ++i) {
+            const int at = (i * 4 + w) * 1024;            // LDS bytes of the wave's transfer
+            // K [plane][chunk][TC][8]: a run of TC cells within the tile's 64
+            const int b = at + lane * 16;
+            lds_dma16_sv(src, (uint32_t)(b / (TC * 16) * 1024 + sub * 16 + b % (TC * 16)), dst + at);
+        }
+#pragma unroll
+        for (int i = 0; i < kHalf / 4096; ++i) {
+            const int at = (i * 4 + w) * 1024;
+            const int b = at + lane * 16, pl = b / (TC * HD * 2), in = b % (TC * HD * 2);
+            lds_dma16_sv(src, (uint32_t)(staged_half<HD, NP>() + pl * 64 * HD * 2 + sub * HD * 2 + in), dst + kHalf + at);
+        }
+    };
+
+    f16v o[RB][DT];
+    float r[RB], l[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        r[b] = -INFINITY;
+        l[b] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[b][d][i] = 0.0f;
+    }
+    int ve = 0;
+    // the wave's own range of positions, for the masks
+    const int64_t rw = min(r0 + (int64_t)w * RB * 32, total - 1);
+    const int pw_lo = base + (int)(rw / g.G), pw_hi = base + (int)(min(r0 + (int64_t)(w + 1) * RB * 32 - 1, total - 1) / g.G);
+    if (k0 < k1) fetch(k0);
+    for (int k = k0; k < k1; ++k) {
+        wait_vmem_all();
+        __syncthreads();
+        if (k + 1 < k1) fetch(k + 1);
+        const int t0 = cell_of(k);
+        const TileInfo ti = info[first + slot_of(t0)];
+        if (!ti.there) continue;
+        const uint8_t *kb = lds + (k & 1) * kStep, *vb = kb + kHalf;
+        if (ti.ve != ve) {                                // V in other units from here on
+            const float f = ldexpf(1.0f, ti.ve - ve);
+            ve = ti.ve;
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[b][d] *= f;
+        }
+        // ---- S^T ----
+        f16v x[RB][CT];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[b][c][i] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                h8v a[NP];
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+                    a[p] = *reinterpret_cast<const h8v *>(kb + p * (TC * HD * 2) + ((2 * ks + half) * TC + c * 32 + n) * 16);
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    if constexpr (NP == 2) {
+                        x[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], qf[0][b][ks], x[b][c], 0, 0, 0);
+                        x[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], qf[1][b][ks], x[b][c], 0, 0, 0);
+                    }
+                    x[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], qf[0][b][ks], x[b][c], 0, 0, 0);
+                }
+            }
+        }
+        // ---- masks, the running reference, the weights ----
+        const bool whole = t0 + TC - 1 <= pw_lo && (t0 > pw_hi - wa.window || t0 + TC <= wa.sinks);
+        h8v pf[NP][RB][CT * 2];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            if (!whole) {
+                const int lo = pos[b] - wa.window;
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int t = t0 + c * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
+                        x[b][c][i] = t <= pos[b] && (t > lo || t < wa.sinks) ? x[b][c][i] : -INFINITY;
+                    }
+            }
+            float mx = x[b][0][0];
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[b][c][i]);
+            mx = swap32_op(mx, [](float p, float q2) { return fmaxf(p, q2); });
+            const float cs = ldexpf(c0[b], -ti.ke), want = mx * cs - kOff;
+            if (__any(want > r[b] + kSlack)) {
+                const float rn = fmaxf(r[b], want), f = __builtin_amdgcn_exp2f(r[b] - (rn == -INFINITY ? 0.0f : rn));
+                r[b] = rn;
+                l[b] *= f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[b][d] *= f;
+            }
+            const float ref = r[b] == -INFINITY ? 0.0f : r[b];
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(x[b][c][i], cs, -ref));
+                    l[b] += e;
+                    pf[0][b][2 * c + (i >> 3)][i & 7] = (_Float16)e;
+                    if constexpr (NP == 2) pf[NP - 1][b][2 * c + (i >> 3)][i & 7] = (_Float16)(e - (float)(_Float16)e);
+                }
+        }
+        // ---- O^T ----
+        if (!ti.odd || whole) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int ks = 0; ks < TC / 16; ++ks) {
+                    h8v a[NP];
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+                        a[p] = *reinterpret_cast<const h8v *>(vb + p * (TC * HD * 2) + ((2 * ks + half) * HD + 32 * d + n) * 16);
+#pragma unroll
+                    for (int b = 0; b < RB; ++b) {
+                        if constexpr (NP == 2) {
+                            o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], pf[0][b][ks], o[b][d], 0, 0, 0);
+                            o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[1][b][ks], o[b][d], 0, 0, 0);
+                        }
+                        o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[0][b][ks], o[b][d], 0, 0, 0);
+                    }
+                }
+        } else {
+            // values that are not finite, which some row does not see: they are left out of the
+            // products, and a row that does see one gets a NaN there
+#pragma unroll 1
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    f16v cnt, add;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) cnt[i] = add[i] = 0.0f;
+#pragma unroll
+                    for (int ks = 0; ks < TC / 16; ++ks) {
+                        const int lo = pos[b] - wa.window;
+                        h8v a[NP], bad, vis;
+#pragma unroll
+                        for (int p = 0; p < NP; ++p)
+                            a[p] = *reinterpret_cast<const h8v *>(vb + p * (TC * HD * 2) + ((2 * ks + half) * HD + 32 * d + n) * 16);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int t = t0 + 16 * ks + 8 * (i >> 2) + 4 * half + (i & 3);
+                            const bool fin = fabsf((float)a[0][i]) < INFINITY;
+                            bad[i] = fin ? (_Float16)0.0f : (_Float16)1.0f;
+                            vis[i] = t <= pos[b] && (t > lo || t < wa.sinks) ? (_Float16)1.0f : (_Float16)0.0f;
+                            a[0][i] = fin ? a[0][i] : (_Float16)0.0f;
+                        }
+                        cnt = __builtin_amdgcn_mfma_f32_32x32x16_f16(bad, vis, cnt, 0, 0, 0);
+                        add = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[0][b][ks], add, 0, 0, 0);
+                        if constexpr (NP == 2) {
+                            add = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], pf[0][b][ks], add, 0, 0, 0);
+                            add = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[1][b][ks], add, 0, 0, 0);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) add[i] = cnt[i] > 0.0f ? NAN : add[i];
+#pragma unroll
+                    for (int dd = 0; dd < DT; ++dd)       // (registers are not indexed by a loop's variable)
+                        if (dd == d) o[b][dd] += add;
+                }
+        }
+    }
+
+    // ---- out ----
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const float ls = swap32_op(l[b], [](float p, float q2) { return p + q2; });
+        if (io[b] < 0) continue;
+        const float f = ldexpf(1.0f, -ve) * (parts == 1 ? (ls != 0.0f ? 1.0f / ls : 0.0f) : 1.0f);
+        const int64_t row = io[b] / HD, pr = ((row / g.H * g.Hkv + gh) * parts + part) * g.G + row % g.G;
+        if (parts > 1 && half == 0) part_rl[pr] = make_float2(r[b], ls);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f4v y = {o[b][d][4 * i], o[b][d][4 * i + 1], o[b][d][4 * i + 2], o[b][d][4 * i + 3]};
+                y *= f;
+                const int at = 32 * d + 8 * i + 4 * half;
+                if (parts > 1) *reinterpret_cast<f4v *>(part_o + pr * HD + at) = y;
+                else store4(wa.out, wa.dtype, io[b] + at, y);
+            }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+static int planes(const WinPlan &p) { return p.dtype == QWFN_SRC_BF16 ? 1 : kExact; }
+static constexpr int rows_a_block() { return 128; }
+
+static PfLayout pf_layout(const Geo &g, const WinPlan &p) {
+    PfLayout l;
+    const int rows = rows_a_block();
+    l.cap = win_most_tiles(p);
+    const int64_t blocks = (int64_t)p.n_rows * g.G / rows + p.n_seq;
+    l.blocks = (int)blocks;
+    // few blocks: their tiles over several workgroups, at least two tiles each
+    const int64_t wgs = blocks * g.Hkv;
+    l.parts = (int)std::max<int64_t>(1, std::min<int64_t>(l.cap / 2, 512 / wgs));
+    size_t off = win_align((size_t)p.n_seq * g.Hkv * l.cap * (size_t)(planes(p) * 64 * g.hd * 2) * 2);
+    auto take = [&](size_t bytes) { const size_t o = off; off = win_align(off + bytes); return o; };
+    l.info = take((size_t)p.n_seq * g.Hkv * l.cap * sizeof(TileInfo));
+    const size_t pr = l.parts > 1 ? (size_t)p.n_rows * g.Hkv * l.parts * g.G : 0;
+    l.part_o = take(pr * g.hd * sizeof(float));
+    l.part_rl = take(pr * sizeof(float2));
+    l.total = off;
+    return l;
+}
+
+template <int HD, int KT, bool VD, int NP>
+static void stage_t(const Geo &g, const qwfn_kv_view &v, const WinArg &wa, const PfLayout &l, uint8_t *ws, hipStream_t st) {
+    hipLaunchKernelGGL((k_win_stage<HD, KT, VD, NP>), dim3((unsigned)l.cap, (unsigned)g.Hkv, (unsigned)wa.n_seq), dim3(256),
+                       0, st, g, v, wa, l.cap, ws, (TileInfo *)(ws + l.info));
+}
+
+template <int HD, int NP, int TC, int RB>
+static hipError_t prefill_t(const Geo &g, const qwfn_kv_view &v, const WinArg &wa, const PfLayout &l, uint8_t *ws, hipStream_t st) {
+    if (g.kt == QWFN_KV_Q4_0) stage_t<HD, QWFN_KV_Q4_0, false, NP>(g, v, wa, l, ws, st);
+    else if (g.kt == QWFN_KV_F16) stage_t<HD, QWFN_KV_F16, false, NP>(g, v, wa, l, ws, st);
+    else if (g.vdim) stage_t<HD, QWFN_KV_Q8_0, true, NP>(g, v, wa, l, ws, st);
+    else stage_t<HD, QWFN_KV_Q8_0, false, NP>(g, v, wa, l, ws, st);
+    constexpr int kLds = 2 * 2 * NP * TC * HD * 2;
+    const hipError_t e = hipFuncSetAttribute((const void *)k_win_rows<HD, NP, TC, RB>,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((k_win_rows<HD, NP, TC, RB>), dim3((unsigned)(l.blocks * l.parts), (unsigned)g.Hkv), dim3(256), kLds,
+                       st, g, v, wa, l.cap, l.parts, ws, (const TileInfo *)(ws + l.info), (float *)(ws + l.part_o),
+                       (float2 *)(ws + l.part_rl));
+    if (l.parts > 1) launch_win_merge(g, wa, l.parts, (const float *)(ws + l.part_o), (const float2 *)(ws + l.part_rl), st);
+    return hipGetLastError();
+}
+
+// A query a sequence at most: the single-token kernels serve it.
+static bool single(const WinPlan &p) { return !p.prefill || p.max_q == 1; }
+
+size_t window_ws_bytes(const Geo &g, const WinPlan &p) { return single(p) ? win_dec_ws_bytes(g, p) : pf_layout(g, p).total; }
 
 hipError_t launch_window(const Geo &g, const qwfn_kv_view &v, const WinArg &wa, const WinPlan &p, void *ws,
                          hipStream_t st) {
-    if (!p.prefill) return launch_win_dec(g, v, wa, p, ws, st);
-    hipLaunchKernelGGL(k_window, dim3((unsigned)p.n_rows, (unsigned)g.H), dim3(256), 0, st, g, v, wa);
-    return hipGetLastError();
+    if (single(p)) return launch_win_dec(g, v, wa, p, ws, st);
+    const PfLayout l = pf_layout(g, p);
+    uint8_t *b = (uint8_t *)ws;
+    const bool exact = planes(p) == kExact;
+    switch (g.hd) {
+    case 64: return exact ? prefill_t<64, 2, 64, 1>(g, v, wa, l, b, st) : prefill_t<64, 1, 64, 1>(g, v, wa, l, b, st);
+    case 128: return exact ? prefill_t<128, 2, 32, 1>(g, v, wa, l, b, st) : prefill_t<128, 1, 64, 1>(g, v, wa, l, b, st);
+    case 256: return exact ? prefill_t<256, 2, 32, 1>(g, v, wa, l, b, st) : prefill_t<256, 1, 32, 1>(g, v, wa, l, b, st);
+    }
+    return hipErrorInvalidValue;
 }
 
 }  // namespace qwfn_qsa

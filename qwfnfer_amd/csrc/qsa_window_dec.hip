@@ -175,17 +175,32 @@ k_win_dec(Geo g, qwfn_kv_view v, WinArg wa, int parts, float *part_o, float2 *pa
     const int hn = lane & 15, lg = lane >> 4, part = blockIdx.x, gh = blockIdx.y, s = blockIdx.z;
     const int head = LOC ? hn & 7 : hn;
     const bool low = LOC && hn >= 8;
+    int row = s, rows = 1;
     const int len = wa.seq_len[s];
-    const bool bad = len < 0 || len > wa.max_seq_len;
+    bool bad = len < 0 || len > wa.max_seq_len;
+    if (wa.q_start) {                                   // a row a sequence at most, anywhere
+        row = wa.q_start[s];
+        rows = wa.q_start[s + 1] - row;
+        if (row < 0 || rows < 0 || rows > wa.n_rows - row) rows = 0, bad = true;
+        bad = bad || rows > 1 || rows > len;
+    }
     const WinTiles tl = win_tiles(bad ? 0 : len, 1, wa.window, wa.sinks);
     if (bad && part == 0 && gh == 0 && threadIdx.x == 0) set_status(v.status, QWFN_STATUS_LEN_RANGE);
+    if (rows != 1) {                                    // none, or too many, which get zeros
+        for (int64_t i = threadIdx.x; i < (int64_t)rows * g.G; i += 256) {
+            const int64_t at = row + i / g.G;
+            if (parts > 1) part_rl[((at * g.Hkv + gh) * parts + part) * g.G + i % g.G] = make_float2(-INFINITY, 0.0f);
+            else for (int d = 0; d < HD; d += 4) store4(wa.out, wa.dtype, (at * g.H + gh * g.G + i % g.G) * HD + d, f4v{0, 0, 0, 0});
+        }
+        return;
+    }
 
     // the column's query: a power of two brings its largest value to [2^13, 2^14), then hi (+ lo)
     h8v qh[NB], ql[LOC ? 1 : NB];
     float qscale;
     {
         float x[NB][8];
-        const int64_t o = ((int64_t)s * g.H + gh * g.G + head) * HD;
+        const int64_t o = ((int64_t)row * g.H + gh * g.G + head) * HD;
         float m = 0.0f;
         if (head < g.G) {
 #pragma unroll
@@ -407,9 +422,9 @@ k_win_dec(Geo g, qwfn_kv_view v, WinArg wa, int parts, float *part_o, float2 *pa
             ls += f * rl[k][h].y;
         }
         if (parts == 1) {
-            store4(wa.out, wa.dtype, ((int64_t)s * g.H + gh * g.G) * HD + at, ls != 0.0f ? y / ls : f4v{0, 0, 0, 0});
+            store4(wa.out, wa.dtype, ((int64_t)row * g.H + gh * g.G) * HD + at, ls != 0.0f ? y / ls : f4v{0, 0, 0, 0});
         } else {
-            const int64_t pr = ((int64_t)(s * g.Hkv + gh) * parts + part) * g.G;
+            const int64_t pr = (((int64_t)row * g.Hkv + gh) * parts + part) * g.G;
             *reinterpret_cast<f4v *>(part_o + pr * HD + at) = y;
             if (at % HD == 0) part_rl[pr + h] = make_float2(rm, ls);
         }
@@ -420,7 +435,8 @@ k_win_dec(Geo g, qwfn_kv_view v, WinArg wa, int parts, float *part_o, float2 *pa
 __global__ void __launch_bounds__(64)
 k_win_merge(Geo g, WinArg wa, int parts, const float *part_o, const float2 *part_rl) {
     const int h = blockIdx.x, gh = h / g.G, row = blockIdx.y, d = threadIdx.x * 4;
-    const int64_t first = ((int64_t)(row * g.Hkv + gh) * parts) * g.G + h % g.G;
+    if (wa.q_start && (row < wa.q_start[0] || row >= wa.q_start[wa.n_seq])) return;
+    const int64_t first = ((int64_t)row * g.Hkv + gh) * parts * g.G + h % g.G;
     float rm = -INFINITY;
     for (int k = 0; k < parts; ++k) rm = fmaxf(rm, part_rl[first + (int64_t)k * g.G].x);
     const float ref = rm == -INFINITY ? 0.0f : rm;
@@ -431,11 +447,17 @@ k_win_merge(Geo g, WinArg wa, int parts, const float *part_o, const float2 *part
         const int64_t at = first + (int64_t)k * g.G;
         const float2 rl = part_rl[at];
         const f4v o = *reinterpret_cast<const f4v *>(part_o + at * g.hd + d);
-        const float f = rl.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(rl.x - ref);
-        y += f * o;                                     // (a part without a tile wrote zeros)
+        const bool none = rl.x == -INFINITY;            // a part without a tile (its o may not be written)
+        const float f = none ? 0.0f : __builtin_amdgcn_exp2f(rl.x - ref);
+        y += none ? f4v{0, 0, 0, 0} : f * o;
         ls += f * rl.y;
     }
     store4(wa.out, wa.dtype, ((int64_t)row * g.H + h) * g.hd + d, ls != 0.0f ? y / ls : f4v{0, 0, 0, 0});
+}
+
+void launch_win_merge(const Geo &g, const WinArg &wa, int parts, const float *part_o, const float2 *part_rl, hipStream_t st) {
+    hipLaunchKernelGGL(k_win_merge, dim3((unsigned)g.H, (unsigned)wa.n_rows), dim3((unsigned)g.hd / 4), 0, st, g, wa, parts,
+                       part_o, part_rl);
 }
 
 // Parts of a sequence's tiles: enough workgroups for two a CU, at most a tile a wave.
@@ -448,7 +470,7 @@ int win_dec_parts(const Geo &g, const WinPlan &p) {
 size_t win_dec_ws_bytes(const Geo &g, const WinPlan &p) {
     const int parts = win_dec_parts(g, p);
     if (parts == 1) return 256;
-    const size_t rows = (size_t)p.n_seq * g.Hkv * parts * g.G;
+    const size_t rows = (size_t)p.n_rows * g.Hkv * parts * g.G;
     return win_align(rows * g.hd * sizeof(float)) + win_align(rows * sizeof(float2));
 }
 
@@ -471,16 +493,14 @@ bool win_shape(int32_t hd, int32_t G) { return G <= 8 ? hd == 64 || hd == 128 ||
 hipError_t launch_win_dec(const Geo &g, const qwfn_kv_view &v, const WinArg &wa, const WinPlan &p, void *ws, hipStream_t st) {
     const int parts = win_dec_parts(g, p);
     float *po = (float *)ws;
-    float2 *rl = (float2 *)((uint8_t *)ws + win_align((size_t)p.n_seq * g.Hkv * parts * g.G * g.hd * sizeof(float)));
+    float2 *rl = (float2 *)((uint8_t *)ws + win_align((size_t)p.n_rows * g.Hkv * parts * g.G * g.hd * sizeof(float)));
     switch (g.hd) {
     case 64: launch_kt<64, true>(g, v, wa, parts, po, rl, st); break;
     case 128: launch_kt<128, true>(g, v, wa, parts, po, rl, st); break;
     case 256: g.G <= 8 ? launch_kt<256, true>(g, v, wa, parts, po, rl, st) : launch_kt<256, false>(g, v, wa, parts, po, rl, st); break;
     default: return hipErrorInvalidValue;
     }
-    if (parts > 1)
-        hipLaunchKernelGGL(k_win_merge, dim3((unsigned)g.H, (unsigned)wa.n_seq), dim3((unsigned)g.hd / 4), 0, st, g, wa,
-                           parts, po, rl);
+    if (parts > 1) launch_win_merge(g, wa, parts, po, rl, st);
     return hipGetLastError();
 }
 

@@ -59,8 +59,9 @@ class Setup:
         return (torch.randn(n, self.cfg.n_head, self.cfg.head_dim, device="cuda", generator=self.gen) * scale).to(dtype)
 
     def expected(self, q, seq, first, window, sinks):
-        """(result, sum p|v|, sum p A (|v| + |o|)) of queries q of sequence seq at positions first ..: A is a
-        logit's sum of magnitudes."""
+        """(result, sum p|v|, sum p A (|v| + |o|), most cells, sum |v|, largest |v|, D) of queries q of sequence seq
+        at positions first ..: A is a logit's sum of magnitudes, D the logits' change where every key value is off
+        by the largest of them."""
         cfg, n = self.cfg, len(q)
         g = cfg.n_head // cfg.n_head_kv
         p = torch.arange(first, first + n, device="cuda")[:, None]
@@ -77,26 +78,37 @@ class Setup:
         o = w @ vv
         b0 = w @ vv.abs()
         b1 = (w * a) @ vv.abs() + (w * a).sum(-1, keepdim=True) * o.abs()
+        sv = (~hidden).double() @ vv.abs()
+        top = vv.abs().amax()
+        d = (qd.abs().sum(-1, keepdim=True) * torch.nan_to_num(k.abs(), nan=0.0, posinf=0.0).amax() / math.sqrt(cfg.head_dim)).expand_as(o)
         back = lambda y: y.permute(2, 0, 1, 3).reshape(n, cfg.n_head, cfg.head_dim)  # noqa: E731
-        return back(o), back(b0), back(b1), int(seen.sum(1).max())
+        return back(o), back(b0), back(b1), int(seen.sum(1).max()), back(sv.expand_as(o)), top, back(d)
 
 
-def check(got, want, dtype, hd):
+def bound_of(want, dtype, hd):
     """Tolerance: a logit is off by at most eps_s of its sum of magnitudes A, which moves the output by at most
     sum p (eps_s A)(|v| + |o|) to first order (the factor 2 covers the rest); weights and values are off by
     eps_v, sums of n terms by n 2^-24 of their magnitudes.
     F32 and F16: operands held to 2^-21 (a sum of two fp16 numbers), fp32 sums: eps_s = (hd + 16) 2^-24 + 2^-19.
-    BF16: keys, values and weights rounded to fp16: eps = 2^-11 each, and the absolute step 2^-25 of the largest
-    value a tile is scaled by.  Then one rounding to the output's type."""
-    o, b0, b1, n = want
+    BF16: keys, values and weights rounded to fp16: eps = 2^-11 each.
+    fp16's step is absolute below 2^-14, half of it 2^-25.  The largest weight is at least 2^13 (BF16: 2^6) of the
+    units the weights are in, so a weight is off by up to 2^-38 (2^-31) of the largest besides, the output by that
+    times sum |v|.  Keys and values are scaled so that a tile's largest is at least 2^7 (BF16: 2^-4): they are off
+    by up to 2^-32 (2^-21) of it besides.  Then one rounding to the output's type."""
+    o, b0, b1, n, sv, top, d = want
     if dtype == torch.bfloat16:
-        eps_s, eps_v = 2.0 ** -11 + (hd + 16) * 2.0 ** -24, 2 * 2.0 ** -11
+        eps_s, eps_v, abs_w, abs_v = 2.0 ** -11 + (hd + 16) * 2.0 ** -24, 2 * 2.0 ** -11, 2.0 ** -31, 2.0 ** -21
     else:
-        eps_s, eps_v = (hd + 16) * 2.0 ** -24 + 2.0 ** -19, 2.0 ** -19
-    out = torch.finfo(dtype).eps / 2
-    bound = 2 * eps_s * b1 + (eps_v + (n + 16) * 2.0 ** -24) * (b0 + o.abs()) + out * o.abs() * 1.01 + 1e-7 * b0 + 2.0 ** -25
+        eps_s, eps_v, abs_w, abs_v = (hd + 16) * 2.0 ** -24 + 2.0 ** -19, 2.0 ** -19, 2.0 ** -38, 2.0 ** -32
+    return (2 * eps_s * b1 + (eps_v + (n + 16) * 2.0 ** -24) * (b0 + o.abs()) + abs_w * sv + abs_v * (top + 2 * d * (b0 + o.abs()))
+            + torch.finfo(dtype).eps / 2 * o.abs() * 1.01)
+
+
+def check(got, want, dtype, hd):
+    """bound_of(), and the absolute half step of a float16 output."""
     assert got.dtype == dtype
-    err = (got.double() - o).abs()
+    o = want[0]
+    err, bound = (got.double() - o).abs(), bound_of(want, dtype, hd) + (2.0 ** -25 if dtype == torch.float16 else 0.0)
     bad = ~(err <= bound)
     assert not bad.any(), (int(bad.sum()), float(err.max()), float((err / bound).max()))
 
@@ -242,7 +254,7 @@ def test_non_finite_cells_out_of_sight(kv, io):
         p = torch.arange(210, 600, device="cuda")
         sees |= (t <= p) & (t > p - window)
     assert sees.any() and not sees.all()
-    check(out[~sees], tuple(x[~sees] for x in o[:3]) + (o[3],), dtype, 128)
+    check(out[~sees], (o[0][~sees], o[1][~sees], o[2][~sees], o[3], o[4][~sees], o[5], o[6][~sees]), dtype, 128)
     # queries that see one: their keys give NaN weights
     assert torch.isnan(out[sees].float()).any(-1).all()
 
@@ -277,23 +289,7 @@ def test_magnitudes(io, kscale, vscale, qscale, kv):
         vscale = min(max(vscale, 1e-5), 5e3)             # what fp16 cells and outputs hold
     st = Setup(config("base", kv), [333, 150], rows=lambda s, k, v: (k * kscale, v * vscale))
     for got, want in _both(st, dtype, qscale):
-        if vscale >= 1:
-            check(got, want, dtype, 128)
-        else:
-            _check_small(got, want, dtype, vscale)
-
-
-def _check_small(got, want, dtype, vscale):
-    """check() of outputs scaled up by a power of two near 1 / vscale, which changes no rounding while the output
-    type's range holds them (fp16: its absolute half step 2^-25 counts)."""
-    o, b0, b1, n = want
-    f = 2.0 ** round(-math.log2(vscale))
-    up = got.double() * f
-    eps_s, eps_v = (2.0 ** -11, 2.0 ** -10) if dtype == torch.bfloat16 else (2.0 ** -19, 2.0 ** -19)
-    out = torch.finfo(dtype).eps / 2
-    bound = f * (2 * (eps_s + 144 * 2.0 ** -24) * b1 + (eps_v + (n + 16) * 2.0 ** -24) * (b0 + o.abs()) + out * 1.01 * o.abs())
-    bound = bound + f * (2.0 ** -25 if dtype == torch.float16 else 0.0) + 1e-6 * f * b0
-    assert ((up - f * o).abs() <= bound).all()
+        check(got, want, dtype, 128)
 
 
 def _both(st, dtype, qscale):
@@ -370,6 +366,26 @@ def test_prefill_bad_sequences():
     assert qsa.read_status(st.cache) == qsa._lib.STATUS_LEN_RANGE
     assert not out[60:].any()
     check(out[:30], st.expected(q[:30], 0, 170, 64, 3), torch.float32, 128)
+
+
+def test_prefill_of_single_rows():
+    """max_q = 1: sequences of a row or none, rows behind the last, and a sequence of two, which is refused."""
+    for lens, window in (([400, 90, 1000, 70], 200), ([9000, 5], 8000)):
+        st = Setup(config("base", 0), lens)
+        n_q = [1, 0, 1, 1] if len(lens) == 4 else [1, 1]
+        for io in ("f32", "bf16"):
+            q, out = prefill(st, n_q, TYPES[io], window, 10, gap=2)
+            check_prefill(st, q, out, n_q, TYPES[io], window, 10)
+            assert qsa.read_status(st.cache) == 0
+        m = len(lens) + 1
+        q = st.queries(m, torch.bfloat16)
+        start = torch.tensor([0, 2, *range(3, m + 1)], dtype=torch.int32, device="cuda")
+        ws = qsa.Workspace.for_window(st.cfg, len(lens), st.max_len, window, 10, n_rows=m, max_q=1, dtype=torch.bfloat16)
+        out = qsa.window_attn_prefill(st.cache, q, start, torch.tensor(lens, dtype=torch.int32, device="cuda"), 1,
+                                      st.max_len, window, ws, sink_tokens=10)
+        assert qsa.read_status(st.cache) == qsa._lib.STATUS_LEN_RANGE
+        assert not out[:2].any()
+        check(out[2:3], st.expected(q[2:3], 1, lens[1] - 1, window, 10), torch.bfloat16, 128)
 
 
 def test_decode_is_the_prefill_of_one_query():
