@@ -9,9 +9,18 @@
 // cached quant is decided by values next to a rounding border, and a far
 // position needs the product pos * turns_i past 24 bits.  The vector pipes run an
 // fp64 fma at the rate of an fp32 one.
+//
+// Two ways.  k_rope_rows8 and k_rope_append8 take rows of 64, 128 or 256 values in
+// 16-byte pieces: a lane holds the two 8-value chunks of a head row whose values
+// turn together, hd / 16 lanes a head row, computes its cos and sin once and goes
+// over several heads with them.  k_rope_rows and k_rope_append take everything
+// else, a wave a head row through LDS.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "qsa_append.h"
+#include "qsa_io.h"
 
 namespace qwfn_qsa {
 
@@ -73,6 +82,115 @@ __device__ __forceinline__ void turn_row(const RopeArg &rp, const float *norm, d
     }
 }
 
+// ---- rows in 16-byte pieces ----
+
+// cos and sin of 2 pi p f, p f exact: the whole turns off, the quarter turns aside,
+// then the Taylor series at |y| <= pi / 4, to y^15 and y^16 (the next terms are below
+// 2^-54).
+__device__ __forceinline__ double2 turn(double p, double f) {
+    const double r = fma(p, f, -rint(p * f)), q = rint(4.0 * r);
+    const double y = fma(-0.25, q, r) * 6.283185307179586476925, z = y * y;
+    double s = -1.0 / 1307674368000.0, c = 1.0 / 20922789888000.0;
+    s = fma(s, z, 1.0 / 6227020800.0);
+    c = fma(c, z, -1.0 / 87178291200.0);
+    s = fma(s, z, -1.0 / 39916800.0);
+    c = fma(c, z, 1.0 / 479001600.0);
+    s = fma(s, z, 1.0 / 362880.0);
+    c = fma(c, z, -1.0 / 3628800.0);
+    s = fma(s, z, -1.0 / 5040.0);
+    c = fma(c, z, 1.0 / 40320.0);
+    s = fma(s, z, 1.0 / 120.0);
+    c = fma(c, z, -1.0 / 720.0);
+    s = fma(s, z, -1.0 / 6.0);
+    c = fma(c, z, 1.0 / 24.0);
+    s = fma(s * z, y, y);
+    c = fma(c, z, -0.5);
+    c = fma(c, z, 1.0);
+    const int k = (int)q & 3;
+    const double a = k & 1 ? s : c, b = k & 1 ? c : s;    // |cos|, |sin|
+    return make_double2(k == 1 || k == 2 ? -a : a, k >= 2 ? -b : b);
+}
+
+// v of lane l ^ 1, 2, 4, 8 (by halves on the DPP network).
+template <int CTRL>
+__device__ __forceinline__ double dppd(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)dppi<CTRL>((int)(uint32_t)u, (int)(uint32_t)u);
+    const uint32_t hi = (uint32_t)dppi<CTRL>((int)(u >> 32), (int)(u >> 32));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// A lane's place in a head row of HD values: chunks a and b of 8 values.  HALF: while the
+// rotation lasts, b is the chunk a turns with.  LH lanes a head row.
+template <int HD, bool IL>
+struct Place {
+    static constexpr int LH = HD / 16;
+    int e, a, b;
+    bool ta, tb;                                          // the chunk turns
+    __device__ __forceinline__ Place(int lane, int rd) {
+        e = lane % LH;
+        if (IL) {
+            a = e;
+            b = e + LH;
+            ta = 8 * a < rd;
+            tb = 8 * b < rd;
+        } else {
+            const int n = rd / 16;                        // lanes whose chunks turn
+            ta = tb = e < n;
+            a = ta ? e : 2 * n + (e - n);
+            b = ta ? e + n : a + (LH - n);
+        }
+    }
+};
+
+// A lane's cos and sin: IL: of chunk a's four pairs and b's; HALF: of the eight pairs of a and b.
+template <int HD, bool IL>
+__device__ __forceinline__ void place_cs(const Place<HD, IL> &pl, const RopeArg &rp, int pos, double2 (&cs)[8]) {
+    const double p = (double)pos;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        cs[k] = make_double2(0.0, 0.0);
+        if (k < 4 || !IL ? pl.ta : pl.tb) {
+            const int i = IL ? 4 * (k < 4 ? pl.a : pl.b) + (k & 3) : 8 * pl.a + k;
+            const double2 t = turn(p, rp.turns[i]);
+            cs[k] = make_double2(t.x * rp.mscale, (rp.inverse ? -t.y : t.y) * rp.mscale);
+        }
+    }
+}
+
+// The lane's 16 values x (chunk a's, then b's) of a head row, normed with w (when NORM) and
+// turned, rounded to fp32 in place.
+template <int HD, bool IL, bool NORM>
+__device__ __forceinline__ void turn16(const Place<HD, IL> &pl, float (&x)[16], const float (&w)[16], const double2 (&cs)[8],
+                                       double eps) {
+    double f = 1.0;
+    if constexpr (NORM) {
+        double ss = 0.0, st = 0.0;
+#pragma unroll
+        for (int k = 0; k < 16; k += 2) {
+            ss = fma((double)x[k], (double)x[k], ss);
+            st = fma((double)x[k + 1], (double)x[k + 1], st);
+        }
+        ss += st;
+        ss += dppd<kDppQuadXor1>(ss);
+        ss += dppd<kDppQuadXor2>(ss);
+        if constexpr (HD >= 128) ss += dppd<kDppRowHalfMirror>(ss);
+        if constexpr (HD >= 256) ss += dppd<kDppRowMirror>(ss);
+        f = 1.0 / sqrt(fma(ss, 1.0 / HD, eps));
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int i = IL ? 2 * k : k, j = IL ? i + 1 : k + 8;
+        double p = (double)x[i], q = (double)x[j];
+        if constexpr (NORM) { p *= (double)w[i]; q *= (double)w[j]; }
+        const bool on = IL && k >= 4 ? pl.tb : pl.ta;     // (a product with 0 would spread a NaN to the other chunk)
+        double y = on ? fma(p, cs[k].x, -(q * cs[k].y)) : p, z = on ? fma(q, cs[k].x, p * cs[k].y) : q;
+        if constexpr (NORM) { y *= f; z *= f; }
+        x[i] = (float)y;
+        x[j] = (float)z;
+    }
+}
+
 }  // namespace
 
 // One wave a head row: item = row * heads + head.
@@ -131,8 +249,300 @@ k_rope_append(Geo g, qwfn_kv_view v, RopeArg rp, RowsArg q, RowsArg k, RowsArg v
                          [&](int d, float *x) { x[0] = y[d]; x[1] = y[d + 1]; x[2] = y[d + 2]; x[3] = y[d + 3]; });
 }
 
+// Rows of HD values in 16-byte pieces: grid (row blocks, head groups), a wave 64 / LH rows
+// at a time, HG heads with one cos and sin.
+constexpr int kHeadGroup = 4;
+constexpr int kKeyGroup = 2;
+
+template <int HD, bool IL, bool NORM>
+__device__ __forceinline__ void rope_heads8(const RopeArg &rp, const RowsArg &src, const float *norm, const int32_t *pos,
+                                            int64_t row0, int64_t n_rows, int h0, int h1, const RowsArg &dst) {
+    const int lane = threadIdx.x & 63;
+    const Place<HD, IL> pl(lane, rp.rd);
+    const int64_t r = row0 + lane / pl.LH, rr = min(r, n_rows - 1);
+    double2 cs[8];
+    place_cs(pl, rp, pos[rr], cs);
+    float w[16];
+    if constexpr (NORM) {
+        load8(norm, QWFN_SRC_F32, 8 * pl.a, w);
+        load8(norm, QWFN_SRC_F32, 8 * pl.b, w + 8);
+    }
+    for (int h = h0; h < h1; ++h) {
+        float x[16];
+        const int64_t at = rr * src.row_stride + h * src.head_stride, to = rr * dst.row_stride + h * dst.head_stride;
+        load8(src.data, src.dtype, at + 8 * pl.a, x);
+        load8(src.data, src.dtype, at + 8 * pl.b, x + 8);
+        turn16<HD, IL, NORM>(pl, x, w, cs, rp.eps);
+        if (r < n_rows) {
+            store8(dst.data, dst.dtype, to + 8 * pl.a, x);
+            store8(dst.data, dst.dtype, to + 8 * pl.b, x + 8);
+        }
+    }
+}
+
+template <int HD, bool IL, bool NORM>
+__global__ void __launch_bounds__(256)
+k_rope_rows8(RopeArg rp, RowsArg src, const float *norm, const int32_t *pos, int64_t n_rows, int heads, RowsArg dst) {
+    constexpr int kRowsWave = 64 * 16 / HD;
+    const int w = threadIdx.x >> 6, h0 = blockIdx.y * kHeadGroup;
+    const int64_t row0 = ((int64_t)blockIdx.x * 4 + w) * kRowsWave;
+    if (row0 < n_rows) rope_heads8<HD, IL, NORM>(rp, src, norm, pos, row0, n_rows, h0, min(h0 + kHeadGroup, heads), dst);
+}
+
+// Where row r's K and V go: its page and row in it; false (and reported once, with `report`) for a
+// bad sequence, position or page.
+struct Dest { int32_t page, row; };
+__device__ __forceinline__ bool dest_of(const Geo &g, const qwfn_kv_view &v, int seq, int t, bool report, Dest &d) {
+    int32_t bad = 0;
+    if (seq < 0 || seq >= g.n_seq_view) bad = QWFN_STATUS_SEQ_RANGE;
+    else if (t < 0 || (int64_t)t >= (int64_t)g.pps * g.pt) bad = QWFN_STATUS_POS_RANGE;
+    else if ((d.page = phys_page(g, v.page_table, seq, t)) < 0) bad = QWFN_STATUS_PAGE_RANGE;
+    if (bad && report) set_status(v.status, bad);
+    d.row = bad ? 0 : t % g.pt;
+    return !bad;
+}
+
+// q8_0 of a 32-value block held by a quad of lanes, 8 values each, as quant4 computes it.
+__device__ __forceinline__ uint2 quad_q8(const float *x, int variant, uint16_t *dh) {
+#pragma clang fp contract(off)
+    float a = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float ax = fabsf(x[k]);
+        a = ax > a ? ax : a;
+    }
+    a = fmaxf(a, dppf<kDppQuadXor1>(a, a));
+    a = fmaxf(a, dppf<kDppQuadXor2>(a, a));
+    const float d = a / 127.0f;
+    *dh = f2h(d);
+    const float id = variant == QWFN_Q8_X86_RNE ? (a != 0.0f ? 127.0f / a : 0.0f) : (d != 0.0f ? 1.0f / d : 0.0f);
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float y = x[k] * id;
+        w[k / 4] |= (uint32_t)(uint8_t)to_i8(variant == QWFN_Q8_X86_RNE ? __builtin_rintf(y) : roundf(y)) << (8 * (k & 3));
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+// q4_0 of a quad's block, as quant_q4 computes it (the first value of the largest magnitude
+// sets the scale): the quants of the lane's 8 values, a byte each; lane e of the quad.
+__device__ __forceinline__ uint2 quad_q4(const float *x, int e, uint16_t *dh) {
+#pragma clang fp contract(off)
+    float a = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a = fmaxf(a, fabsf(x[k]));
+    a = fmaxf(a, dppf<kDppQuadXor1>(a, a));
+    a = fmaxf(a, dppf<kDppQuadXor2>(a, a));
+    int bi = 32;
+    float bv = 0.0f;
+#pragma unroll
+    for (int k = 7; k >= 0; --k)
+        if (a > 0.0f && fabsf(x[k]) == a) { bi = 8 * e + k; bv = x[k]; }
+#pragma unroll
+    for (int step = 0; step < 2; ++step) {
+        const int oi = step ? dppi<kDppQuadXor2>(bi, bi) : dppi<kDppQuadXor1>(bi, bi);
+        const float ov = step ? dppf<kDppQuadXor2>(bv, bv) : dppf<kDppQuadXor1>(bv, bv);
+        if (oi < bi) { bi = oi; bv = ov; }
+    }
+    const float d = bv / -8.0f;
+    *dh = f2h(d);
+    const float id = d != 0.0f ? 1.0f / d : 0.0f;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float y = x[k] * id + 8.5f;
+        const int t = y != y ? 0 : (int)y;
+        w[k / 4] |= (uint32_t)(t < 15 ? t : 15) << (8 * (k & 3));
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+// Chunk c (8 values, four lanes of a quad holding chunks 4 j .. 4 j + 3) of a head row into a
+// K-layout page.  The quad is together; `live` is the same in it.
+template <int KT>
+__device__ __forceinline__ void store_chunk(const Geo &g, uint8_t *page, int gh, int row, int c, const float *x, bool live) {
+    if constexpr (KT == QWFN_KV_F16) {
+        if (live) store8(page + chunk_off(g, gh, row, c), QWFN_SRC_F16, 0, x);
+    } else {
+        uint16_t dh;
+        if constexpr (KT == QWFN_KV_Q4_0) {
+            const uint2 w = quad_q4(x, c & 3, &dh);
+            // dims 0 .. 15 of the block in the low nibbles, 16 .. 31 in the high ones
+            const uint32_t hx = (uint32_t)dppi<kDppQuadXor2>((int)w.x, (int)w.x), hy = (uint32_t)dppi<kDppQuadXor2>((int)w.y, (int)w.y);
+            if (live && (c & 3) < 2)
+                *reinterpret_cast<uint2 *>(page + chunk_off(g, gh, row, c / 4) + 8 * (c & 1)) = make_uint2(w.x | hx << 4, w.y | hy << 4);
+        } else {
+            const uint2 w = quad_q8(x, g.variant, &dh);
+            if (live) *reinterpret_cast<uint2 *>(page + quant_off(g, gh, row, 8 * c)) = w;
+        }
+        if (live && (c & 3) == 0) *reinterpret_cast<uint16_t *>(page + scale_off(g, gh, row, c / 4)) = dh;
+    }
+}
+
+template <int HD, bool IL, bool NORM, int KT>
+__device__ __forceinline__ void keys8(const Geo &g, const qwfn_kv_view &v, const RopeArg &rp, const RowsArg &k,
+                                      const float *norm, const int32_t *seq_ids, const int32_t *pos, int64_t row0,
+                                      int64_t n_rows, int h0, int h1) {
+    const int lane = threadIdx.x & 63;
+    const Place<HD, IL> pl(lane, rp.rd);
+    const int64_t r = row0 + lane / pl.LH, rr = min(r, n_rows - 1);
+    const int t = pos[rr];
+    Dest d;
+    const bool live = dest_of(g, v, seq_ids ? seq_ids[rr] : 0, t, h0 == 0 && pl.e == 0 && r < n_rows, d) && r < n_rows;
+    uint8_t *page = (uint8_t *)v.k_pages + (live ? (int64_t)d.page * g.page_bytes : 0);
+    double2 cs[8];
+    place_cs(pl, rp, t, cs);
+    float w[16];
+    if constexpr (NORM) {
+        load8(norm, QWFN_SRC_F32, 8 * pl.a, w);
+        load8(norm, QWFN_SRC_F32, 8 * pl.b, w + 8);
+    }
+    for (int h = h0; h < h1; ++h) {
+        float x[16];
+        const int64_t at = rr * k.row_stride + h * k.head_stride;
+        load8(k.data, k.dtype, at + 8 * pl.a, x);
+        load8(k.data, k.dtype, at + 8 * pl.b, x + 8);
+        turn16<HD, IL, NORM>(pl, x, w, cs, rp.eps);
+        store_chunk<KT>(g, page, h, d.row, pl.a, x, live);
+        store_chunk<KT>(g, page, h, d.row, pl.b, x + 8, live);
+    }
+}
+
+// The V rows of a K-layout page: chunks e and e + LH of a lane.
+template <int HD, int KT>
+__device__ __forceinline__ void values8(const Geo &g, const qwfn_kv_view &v, const RowsArg &vv, const int32_t *seq_ids,
+                                        const int32_t *pos, int64_t row0, int64_t n_rows, int h) {
+    constexpr int LH = HD / 16;
+    const int lane = threadIdx.x & 63, e = lane % LH;
+    const int64_t r = row0 + lane / LH, rr = min(r, n_rows - 1);
+    Dest d;
+    const bool live = dest_of(g, v, seq_ids ? seq_ids[rr] : 0, pos[rr], false, d) && r < n_rows;
+    uint8_t *page = (uint8_t *)v.v_pages + (live ? (int64_t)d.page * g.page_bytes : 0);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        float x[8];
+        load8(vv.data, vv.dtype, rr * vv.row_stride + h * vv.head_stride + 8 * (e + k * LH), x);
+        store_chunk<KT>(g, page, h, d.row, e + k * LH, x, live);
+    }
+}
+
+// The V rows of a q8_0 page that is dimension-major in its 64-token tiles: a workgroup's 64
+// rows of one head are quantized by rows and turned in LDS.  Rows at positions that follow
+// each other (a prompt's) leave it as whole words, others byte by byte.
+constexpr int kTurnRow = 68;                              // 64 bytes of a dimension, displaced by up to 3
+template <int HD>
+__device__ __forceinline__ void values_turned(const Geo &g, const qwfn_kv_view &v, const RowsArg &vv, const int32_t *seq_ids,
+                                              const int32_t *pos, int64_t row0, int64_t n_rows, int h, uint8_t *lds) {
+    constexpr int LH = HD / 16, kRowsWave = 64 / LH;
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, e = lane % LH, tid = threadIdx.x;
+    const int m = (int)min((int64_t)64, n_rows - row0);
+    const int t0 = pos[row0], s0 = seq_ids ? seq_ids[row0] : 0;
+    bool run = t0 >= 0 && (int64_t)t0 + m <= (int64_t)g.pps * g.pt && s0 >= 0 && s0 < g.n_seq_view;
+    if (tid < m) run = run && (int64_t)pos[row0 + tid] == (int64_t)t0 + tid && (!seq_ids || seq_ids[row0 + tid] == s0);
+    run = __syncthreads_and(run);
+    const int a = run ? t0 & 3 : 0;
+    for (int i = wv * kRowsWave; i < m; i += 4 * kRowsWave) {
+        const int o = i + lane / LH;
+        const int64_t rr = row0 + min(o, m - 1);
+        Dest d;
+        const bool live = dest_of(g, v, seq_ids ? seq_ids[rr] : 0, pos[rr], false, d) && o < m;
+        uint8_t *page = (uint8_t *)v.v_pages + (live ? (int64_t)d.page * g.page_bytes : 0);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int c = e + k * LH;
+            float x[8];
+            load8(vv.data, vv.dtype, rr * vv.row_stride + h * vv.head_stride + 8 * c, x);
+            uint16_t dh;
+            const uint2 w = quad_q8(x, g.variant, &dh);
+            if (live && (c & 3) == 0) *reinterpret_cast<uint16_t *>(page + scale_off(g, h, d.row, c / 4)) = dh;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint8_t b = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
+                if (run) {
+                    if (o < m) lds[(8 * c + j) * kTurnRow + a + o] = b;
+                } else if (live) {
+                    page[vquant_off(g, h, d.row, 8 * c + j)] = b;
+                }
+            }
+        }
+    }
+    if (!run) return;
+    __syncthreads();
+    // word k of a dimension: cells t0 - a + 4 k .. + 3, which lie in one tile
+    for (int i = tid; i < HD * 17; i += 256) {
+        const int dim = i / 17, k = i % 17, c0 = 4 * k - a, t = t0 + c0;
+        if (c0 >= m) continue;
+        const int32_t pp = phys_page(g, v.page_table, s0, t);
+        if (pp < 0) continue;
+        uint8_t *to = (uint8_t *)v.v_pages + (int64_t)pp * g.page_bytes + vquant_off(g, h, t % g.pt, dim);
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(lds + dim * kTurnRow + 4 * k);
+        if (c0 >= 0 && c0 + 4 <= m) {
+            *reinterpret_cast<uint32_t *>(to) = w;
+        } else {
+            for (int j = 0; j < 4; ++j)
+                if (c0 + j >= 0 && c0 + j < m) to[j] = (uint8_t)(w >> (8 * j));
+        }
+    }
+}
+
+// Q, K and V of 64 rows: grid (ceil(rows / 64), groups of query heads, then of key heads, then
+// one a value head).
+template <int HD, int KT, bool IL>
+__global__ void __launch_bounds__(256)
+k_rope_append8(Geo g, qwfn_kv_view v, RopeArg rp, RowsArg q, RowsArg k, RowsArg vv, const float *q_norm,
+               const float *k_norm, const int32_t *seq_ids, const int32_t *pos, int64_t n_rows, int n_q, RowsArg q_out) {
+    constexpr int kRowsWave = 64 * 16 / HD;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[KT == QWFN_KV_Q8_0 ? HD * kTurnRow : 16];
+    const int qg = (n_q + kHeadGroup - 1) / kHeadGroup, kg = (g.Hkv + kKeyGroup - 1) / kKeyGroup;
+    const int64_t b0 = (int64_t)blockIdx.x * 64, b1 = min(b0 + 64, n_rows);
+    const int role = blockIdx.y;
+    if (KT == QWFN_KV_Q8_0 && role >= qg + kg && g.vdim) {
+        values_turned<HD>(g, v, vv, seq_ids, pos, b0, n_rows, role - qg - kg, lds);
+        return;
+    }
+    for (int64_t r = b0 + (threadIdx.x >> 6) * kRowsWave; r < b1; r += 4 * kRowsWave) {
+        if (role < qg) {
+            const int h0 = role * kHeadGroup, h1 = min(h0 + kHeadGroup, n_q);
+            if (q_norm) rope_heads8<HD, IL, true>(rp, q, q_norm, pos, r, n_rows, h0, h1, q_out);
+            else rope_heads8<HD, IL, false>(rp, q, nullptr, pos, r, n_rows, h0, h1, q_out);
+        } else if (role < qg + kg) {
+            const int h0 = (role - qg) * kKeyGroup, h1 = min(h0 + kKeyGroup, g.Hkv);
+            if (k_norm) keys8<HD, IL, true, KT>(g, v, rp, k, k_norm, seq_ids, pos, r, n_rows, h0, h1);
+            else keys8<HD, IL, false, KT>(g, v, rp, k, nullptr, seq_ids, pos, r, n_rows, h0, h1);
+        } else {
+            values8<HD, KT>(g, v, vv, seq_ids, pos, r, n_rows, role - qg - kg);
+        }
+    }
+}
+
+// Rows that begin, every one, at a 16-byte boundary.
+static bool pieces(const RowsArg &r) {
+    const int64_t n = r.dtype == QWFN_SRC_F32 ? 4 : 8;
+    return (uintptr_t)r.data % 16 == 0 && r.row_stride % n == 0 && r.head_stride % n == 0;
+}
+// A rotation whose pairs lie in a chunk, or in two whole chunks.
+static bool pieces_fit(const RopeArg &rp, int hd) {
+    return (hd == 64 || hd == 128 || hd == 256) && rp.rd % (rp.interleaved ? 8 : 16) == 0;
+}
+
 hipError_t launch_rope_rows(const RopeArg &rp, const RowsArg &src, const float *norm, const int32_t *pos,
                             int32_t n_rows, int32_t heads, int32_t hd, const RowsArg &dst, hipStream_t st) {
+    if (pieces_fit(rp, hd) && pieces(src) && pieces(dst) && (!norm || (uintptr_t)norm % 16 == 0)) {
+        const auto go = [&](auto kern) {
+            const int rows = 4 * 64 * 16 / hd;
+            hipLaunchKernelGGL(kern, dim3((unsigned)((n_rows + rows - 1) / rows), (unsigned)((heads + kHeadGroup - 1) / kHeadGroup)),
+                               dim3(256), 0, st, rp, src, norm, pos, n_rows, heads, dst);
+            return hipGetLastError();
+        };
+        const auto of = [&](auto hdc) {
+            constexpr int HD = decltype(hdc)::value;
+            if (rp.interleaved) return norm ? go(k_rope_rows8<HD, true, true>) : go(k_rope_rows8<HD, true, false>);
+            return norm ? go(k_rope_rows8<HD, false, true>) : go(k_rope_rows8<HD, false, false>);
+        };
+        return hd == 64 ? of(std::integral_constant<int, 64>()) : hd == 128 ? of(std::integral_constant<int, 128>())
+                                                                            : of(std::integral_constant<int, 256>());
+    }
     const int64_t items = (int64_t)n_rows * heads;
     hipLaunchKernelGGL(k_rope_rows, dim3((unsigned)((items + kWaves - 1) / kWaves)), dim3(64 * kWaves), 0, st, rp, src,
                        norm, pos, items, heads, hd, dst);
@@ -144,6 +554,28 @@ hipError_t launch_rope_append(const Geo &g, const qwfn_kv_view &v, const RopeArg
                               const int32_t *seq_ids, const int32_t *pos, int32_t n_rows, const RowsArg &q_out,
                               hipStream_t st) {
     const int n_q = q.data ? g.H : 0;
+    // quantized blocks of 32 are a quad of lanes' chunks: whole, when half the rotated values are
+    const bool quads = g.kt == QWFN_KV_F16 || rp.interleaved || rp.rd % 64 == 0;
+    const auto whole = [](const float *w) { return (uintptr_t)w % 16 == 0; };
+    if (quads && pieces_fit(rp, g.hd) && pieces(k) && pieces(vv) && (!n_q || (pieces(q) && pieces(q_out))) && whole(q_norm) &&
+        whole(k_norm)) {
+        const unsigned roles = (n_q + kHeadGroup - 1) / kHeadGroup + (g.Hkv + kKeyGroup - 1) / kKeyGroup + g.Hkv;
+        const auto go = [&](auto kern) {
+            hipLaunchKernelGGL(kern, dim3((unsigned)(((int64_t)n_rows + 63) / 64), roles), dim3(256), 0, st, g, v, rp, q, k,
+                               vv, q_norm, k_norm, seq_ids, pos, n_rows, n_q, q_out);
+            return hipGetLastError();
+        };
+        const auto of = [&](auto hdc) {
+            constexpr int HD = decltype(hdc)::value;
+            if (g.kt == QWFN_KV_Q4_0)
+                return rp.interleaved ? go(k_rope_append8<HD, QWFN_KV_Q4_0, true>) : go(k_rope_append8<HD, QWFN_KV_Q4_0, false>);
+            if (g.kt == QWFN_KV_F16)
+                return rp.interleaved ? go(k_rope_append8<HD, QWFN_KV_F16, true>) : go(k_rope_append8<HD, QWFN_KV_F16, false>);
+            return rp.interleaved ? go(k_rope_append8<HD, QWFN_KV_Q8_0, true>) : go(k_rope_append8<HD, QWFN_KV_Q8_0, false>);
+        };
+        return g.hd == 64 ? of(std::integral_constant<int, 64>()) : g.hd == 128 ? of(std::integral_constant<int, 128>())
+                                                                                : of(std::integral_constant<int, 256>());
+    }
     const int64_t items = (int64_t)n_rows * (n_q + 2 * g.Hkv);
     hipLaunchKernelGGL(k_rope_append, dim3((unsigned)((items + kWaves - 1) / kWaves)), dim3(64 * kWaves), 0, st, g, v,
                        rp, q, k, vv, q_norm, k_norm, seq_ids, pos, items, n_q, q_out);

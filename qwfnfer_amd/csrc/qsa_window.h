@@ -1,10 +1,10 @@
 // qsa_window.h -- what the sliding-window kernels share: a sequence's list of
-// 64-cell tiles, rows of the three element types, the parts' merge.
+// 64-cell tiles, a row's power of two, the parts' merge.
 #pragma once
 
 #include <algorithm>
 
-#include "qsa_device.h"
+#include "qsa_io.h"
 
 namespace qwfn_qsa {
 
@@ -41,36 +41,6 @@ inline int win_most_tiles(const WinPlan &p) {
     const int64_t all = ((int64_t)p.max_seq_len + 63) / 64;
     const int64_t win = ((int64_t)p.window + p.max_q - 1 + 126) / 64, sink = ((int64_t)p.sinks + 63) / 64;
     return (int)std::min<int64_t>(all, win + sink);
-}
-
-__device__ __forceinline__ float bf16_f(uint32_t h) { return __uint_as_float(h << 16); }
-
-// Eight values of a row at a 16-byte (fp32: 32-byte run's) boundary.
-__device__ __forceinline__ void load8(const void *p, int dtype, int64_t i, float *x) {
-    if (dtype == QWFN_SRC_F32) {
-        const f4v a = *reinterpret_cast<const f4v *>((const float *)p + i), b = *reinterpret_cast<const f4v *>((const float *)p + i + 4);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) { x[k] = a[k]; x[4 + k] = b[k]; }
-    } else {
-        const u4v w = *reinterpret_cast<const u4v *>((const uint16_t *)p + i);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            x[2 * k] = dtype == QWFN_SRC_F16 ? h2f((uint16_t)w[k]) : bf16_f(w[k] & 0xFFFFu);
-            x[2 * k + 1] = dtype == QWFN_SRC_F16 ? h2f((uint16_t)(w[k] >> 16)) : bf16_f(w[k] >> 16);
-        }
-    }
-}
-// Four values of a row.
-__device__ __forceinline__ void store4(void *p, int dtype, int64_t i, f4v y) {
-    if (dtype == QWFN_SRC_F32) {
-        *reinterpret_cast<f4v *>((float *)p + i) = y;
-    } else if (dtype == QWFN_SRC_F16) {
-        typedef _Float16 h4v __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<h4v *>((uint16_t *)p + i) = __builtin_convertvector(y, h4v);
-    } else {
-        typedef __bf16 b4v __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<b4v *>((uint16_t *)p + i) = __builtin_convertvector(y, b4v);
-    }
 }
 
 // The exponent e that brings a row's largest magnitude m to [2^k, 2^(k + 1)): x 2^e.  A
