@@ -17,6 +17,7 @@
 // else, a wave a head row through LDS.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "qsa_append.h"
@@ -37,6 +38,14 @@ __device__ __forceinline__ void put_row_value(const RowsArg &r, int64_t i, float
     if (r.dtype == QWFN_SRC_F32) ((float *)r.data)[i] = y;
     else if (r.dtype == QWFN_SRC_F16) ((uint16_t *)r.data)[i] = f2h(y);
     else ((__bf16 *)r.data)[i] = (__bf16)y;
+}
+
+// fp32 of a 64-bit result, a rounding of its own: without the barrier the compiler may join it
+// with a following rounding to fp16 (floating-point contraction), which differs at ties.
+__device__ __forceinline__ float round32(double y) {
+    float f = (float)y;
+    asm("" : "+v"(f));
+    return f;
 }
 
 __device__ __forceinline__ double wave_sum_f64(double v) {
@@ -78,7 +87,7 @@ __device__ __forceinline__ void turn_row(const RopeArg &rp, const float *norm, d
             const double2 cs = rope_cs(rp, pos, i);
             y = second ? y * cs.x + x[o] * cs.y : y * cs.x - x[o] * cs.y;
         }
-        put(d, (float)y);
+        put(d, round32(y));
     }
 }
 
@@ -146,7 +155,7 @@ struct Place {
 // A lane's cos and sin: IL: of chunk a's four pairs and b's; HALF: of the eight pairs of a and b.
 template <int HD, bool IL>
 __device__ __forceinline__ void place_cs(const Place<HD, IL> &pl, const RopeArg &rp, int pos, double2 (&cs)[8]) {
-    const double p = (double)pos;
+    double p = (double)pos;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         cs[k] = make_double2(0.0, 0.0);
@@ -155,16 +164,18 @@ __device__ __forceinline__ void place_cs(const Place<HD, IL> &pl, const RopeArg 
             const double2 t = turn(p, rp.turns[i]);
             cs[k] = make_double2(t.x * rp.mscale, (rp.inverse ? -t.y : t.y) * rp.mscale);
         }
+        // one pair after the other: eight chains at once would take the registers of a wave more a SIMD
+        asm volatile("" : "+v"(p), "+v"(cs[k].x), "+v"(cs[k].y));
     }
 }
 
-// The lane's 16 values x (chunk a's, then b's) of a head row, normed with w (when NORM) and
-// turned, rounded to fp32 in place.
-template <int HD, bool IL, bool NORM>
-__device__ __forceinline__ void turn16(const Place<HD, IL> &pl, float (&x)[16], const float (&w)[16], const double2 (&cs)[8],
-                                       double eps) {
+// The lane's 16 values x (chunk a's, then b's) of a head row, normed (norm: with the weights w)
+// and turned, rounded to fp32 in place.
+template <int HD, bool IL>
+__device__ __forceinline__ void turn16(const Place<HD, IL> &pl, float (&x)[16], bool norm, const float (&w)[16],
+                                       const double2 (&cs)[8], double eps) {
     double f = 1.0;
-    if constexpr (NORM) {
+    if (norm) {
         double ss = 0.0, st = 0.0;
 #pragma unroll
         for (int k = 0; k < 16; k += 2) {
@@ -176,18 +187,15 @@ __device__ __forceinline__ void turn16(const Place<HD, IL> &pl, float (&x)[16], 
         ss += dppd<kDppQuadXor2>(ss);
         if constexpr (HD >= 128) ss += dppd<kDppRowHalfMirror>(ss);
         if constexpr (HD >= 256) ss += dppd<kDppRowMirror>(ss);
-        f = 1.0 / sqrt(fma(ss, 1.0 / HD, eps));
+        f = rsqrt(fma(ss, 1.0 / HD, eps));
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         const int i = IL ? 2 * k : k, j = IL ? i + 1 : k + 8;
-        double p = (double)x[i], q = (double)x[j];
-        if constexpr (NORM) { p *= (double)w[i]; q *= (double)w[j]; }
+        const double p = (double)x[i] * ((double)w[i] * f), q = (double)x[j] * ((double)w[j] * f);
         const bool on = IL && k >= 4 ? pl.tb : pl.ta;     // (a product with 0 would spread a NaN to the other chunk)
-        double y = on ? fma(p, cs[k].x, -(q * cs[k].y)) : p, z = on ? fma(q, cs[k].x, p * cs[k].y) : q;
-        if constexpr (NORM) { y *= f; z *= f; }
-        x[i] = (float)y;
-        x[j] = (float)z;
+        x[i] = round32(on ? fma(p, cs[k].x, -(q * cs[k].y)) : p);
+        x[j] = round32(on ? fma(q, cs[k].x, p * cs[k].y) : q);
     }
 }
 
@@ -249,44 +257,75 @@ k_rope_append(Geo g, qwfn_kv_view v, RopeArg rp, RowsArg q, RowsArg k, RowsArg v
                          [&](int d, float *x) { x[0] = y[d]; x[1] = y[d + 1]; x[2] = y[d + 2]; x[3] = y[d + 3]; });
 }
 
-// Rows of HD values in 16-byte pieces: grid (row blocks, head groups), a wave 64 / LH rows
-// at a time, HG heads with one cos and sin.
-constexpr int kHeadGroup = 4;
-constexpr int kKeyGroup = 2;
+// A lane's two chunks as they lie in memory (loaded a head ahead of their use).
+template <int SZ>
+struct Raw {
+    u4v c[SZ];                                            // 2 chunks of 8 values of SZ bytes
+    __device__ __forceinline__ void load(const RowsArg &r, int64_t at, int a, int b) {
+        const uint8_t *p = (const uint8_t *)r.data + at * SZ;
+#pragma unroll
+        for (int k = 0; k < SZ / 2; ++k) {
+            c[k] = *reinterpret_cast<const u4v *>(p + 8 * SZ * a + 16 * k);
+            c[SZ / 2 + k] = *reinterpret_cast<const u4v *>(p + 8 * SZ * b + 16 * k);
+        }
+    }
+    __device__ __forceinline__ void values(int dtype, float (&x)[16]) const {
+#pragma unroll
+        for (int k = 0; k < 4 * SZ; ++k) {
+            const uint32_t w = c[k >> 2][k & 3];
+            if constexpr (SZ == 4) {
+                x[k] = __uint_as_float(w);
+            } else {
+                x[2 * k] = dtype == QWFN_SRC_F16 ? h2f((uint16_t)w) : bf16_f(w & 0xFFFFu);
+                x[2 * k + 1] = dtype == QWFN_SRC_F16 ? h2f((uint16_t)(w >> 16)) : bf16_f(w >> 16);
+            }
+        }
+    }
+};
 
-template <int HD, bool IL, bool NORM>
-__device__ __forceinline__ void rope_heads8(const RopeArg &rp, const RowsArg &src, const float *norm, const int32_t *pos,
-                                            int64_t row0, int64_t n_rows, int h0, int h1, const RowsArg &dst) {
-    const int lane = threadIdx.x & 63;
-    const Place<HD, IL> pl(lane, rp.rd);
-    const int64_t r = row0 + lane / pl.LH, rr = min(r, n_rows - 1);
-    double2 cs[8];
-    place_cs(pl, rp, pos[rr], cs);
+// Rows of HD values in 16-byte pieces: a wave 64 / LH rows at a time, heads h0 .. h1 - 1 with
+// one cos and sin; put(h, x) takes the lane's 16 results of head h.
+template <int HD, bool IL, int SZ, class Put>
+__device__ __forceinline__ void heads8(const RopeArg &rp, const Place<HD, IL> &pl, const RowsArg &src, const float *norm,
+                                       int64_t rr, int pos, int h0, int h1, Put put) {
+    const int64_t at = rr * src.row_stride;
+    Raw<SZ> next;
+    next.load(src, at + h0 * src.head_stride, pl.a, pl.b);
     float w[16];
-    if constexpr (NORM) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) w[k] = 1.0f;
+    if (norm) {
         load8(norm, QWFN_SRC_F32, 8 * pl.a, w);
         load8(norm, QWFN_SRC_F32, 8 * pl.b, w + 8);
     }
+    double2 cs[8];
+    place_cs(pl, rp, pos, cs);
     for (int h = h0; h < h1; ++h) {
         float x[16];
-        const int64_t at = rr * src.row_stride + h * src.head_stride, to = rr * dst.row_stride + h * dst.head_stride;
-        load8(src.data, src.dtype, at + 8 * pl.a, x);
-        load8(src.data, src.dtype, at + 8 * pl.b, x + 8);
-        turn16<HD, IL, NORM>(pl, x, w, cs, rp.eps);
-        if (r < n_rows) {
-            store8(dst.data, dst.dtype, to + 8 * pl.a, x);
-            store8(dst.data, dst.dtype, to + 8 * pl.b, x + 8);
-        }
+        next.values(src.dtype, x);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) asm("" : "+v"(w[k]));            // (its 64-bit form is not held over the loop)
+        if (h + 1 < h1) next.load(src, at + (h + 1) * src.head_stride, pl.a, pl.b);
+        turn16(pl, x, norm != nullptr, w, cs, rp.eps);
+        put(h, x);
     }
 }
 
-template <int HD, bool IL, bool NORM>
-__global__ void __launch_bounds__(256)
-k_rope_rows8(RopeArg rp, RowsArg src, const float *norm, const int32_t *pos, int64_t n_rows, int heads, RowsArg dst) {
+// grid (row blocks, groups of hg heads).
+template <int HD, bool IL, int SZ>
+__global__ void __launch_bounds__(256, SZ == 4 ? 3 : 4)
+k_rope_rows8(RopeArg rp, RowsArg src, const float *norm, const int32_t *pos, int64_t n_rows, int heads, int hg, RowsArg dst) {
     constexpr int kRowsWave = 64 * 16 / HD;
-    const int w = threadIdx.x >> 6, h0 = blockIdx.y * kHeadGroup;
-    const int64_t row0 = ((int64_t)blockIdx.x * 4 + w) * kRowsWave;
-    if (row0 < n_rows) rope_heads8<HD, IL, NORM>(rp, src, norm, pos, row0, n_rows, h0, min(h0 + kHeadGroup, heads), dst);
+    const int lane = threadIdx.x & 63, h0 = blockIdx.y * hg;
+    const int64_t row0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kRowsWave;
+    if (row0 >= n_rows) return;
+    const Place<HD, IL> pl(lane, rp.rd);
+    const int64_t r = row0 + lane / pl.LH, rr = min(r, n_rows - 1), to = rr * dst.row_stride;
+    heads8<HD, IL, SZ>(rp, pl, src, norm, rr, pos[rr], h0, min(h0 + hg, heads), [&](int h, const float *x) {
+        if (r >= n_rows) return;
+        store8(dst.data, dst.dtype, to + h * dst.head_stride + 8 * pl.a, x);
+        store8(dst.data, dst.dtype, to + h * dst.head_stride + 8 * pl.b, x + 8);
+    });
 }
 
 // Where row r's K and V go: its page and row in it; false (and reported once, with `report`) for a
@@ -380,63 +419,16 @@ __device__ __forceinline__ void store_chunk(const Geo &g, uint8_t *page, int gh,
     }
 }
 
-template <int HD, bool IL, bool NORM, int KT>
-__device__ __forceinline__ void keys8(const Geo &g, const qwfn_kv_view &v, const RopeArg &rp, const RowsArg &k,
-                                      const float *norm, const int32_t *seq_ids, const int32_t *pos, int64_t row0,
-                                      int64_t n_rows, int h0, int h1) {
-    const int lane = threadIdx.x & 63;
-    const Place<HD, IL> pl(lane, rp.rd);
-    const int64_t r = row0 + lane / pl.LH, rr = min(r, n_rows - 1);
-    const int t = pos[rr];
-    Dest d;
-    const bool live = dest_of(g, v, seq_ids ? seq_ids[rr] : 0, t, h0 == 0 && pl.e == 0 && r < n_rows, d) && r < n_rows;
-    uint8_t *page = (uint8_t *)v.k_pages + (live ? (int64_t)d.page * g.page_bytes : 0);
-    double2 cs[8];
-    place_cs(pl, rp, t, cs);
-    float w[16];
-    if constexpr (NORM) {
-        load8(norm, QWFN_SRC_F32, 8 * pl.a, w);
-        load8(norm, QWFN_SRC_F32, 8 * pl.b, w + 8);
-    }
-    for (int h = h0; h < h1; ++h) {
-        float x[16];
-        const int64_t at = rr * k.row_stride + h * k.head_stride;
-        load8(k.data, k.dtype, at + 8 * pl.a, x);
-        load8(k.data, k.dtype, at + 8 * pl.b, x + 8);
-        turn16<HD, IL, NORM>(pl, x, w, cs, rp.eps);
-        store_chunk<KT>(g, page, h, d.row, pl.a, x, live);
-        store_chunk<KT>(g, page, h, d.row, pl.b, x + 8, live);
-    }
-}
-
-// The V rows of a K-layout page: chunks e and e + LH of a lane.
-template <int HD, int KT>
-__device__ __forceinline__ void values8(const Geo &g, const qwfn_kv_view &v, const RowsArg &vv, const int32_t *seq_ids,
-                                        const int32_t *pos, int64_t row0, int64_t n_rows, int h) {
-    constexpr int LH = HD / 16;
-    const int lane = threadIdx.x & 63, e = lane % LH;
-    const int64_t r = row0 + lane / LH, rr = min(r, n_rows - 1);
-    Dest d;
-    const bool live = dest_of(g, v, seq_ids ? seq_ids[rr] : 0, pos[rr], false, d) && r < n_rows;
-    uint8_t *page = (uint8_t *)v.v_pages + (live ? (int64_t)d.page * g.page_bytes : 0);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        float x[8];
-        load8(vv.data, vv.dtype, rr * vv.row_stride + h * vv.head_stride + 8 * (e + k * LH), x);
-        store_chunk<KT>(g, page, h, d.row, e + k * LH, x, live);
-    }
-}
-
-// The V rows of a q8_0 page that is dimension-major in its 64-token tiles: a workgroup's 64
-// rows of one head are quantized by rows and turned in LDS.  Rows at positions that follow
+// The V rows of a q8_0 page that is dimension-major in its 64-token tiles: a workgroup's up
+// to 64 rows of one head are quantized by rows and turned in LDS.  Rows at positions that follow
 // each other (a prompt's) leave it as whole words, others byte by byte.
 constexpr int kTurnRow = 68;                              // 64 bytes of a dimension, displaced by up to 3
 template <int HD>
 __device__ __forceinline__ void values_turned(const Geo &g, const qwfn_kv_view &v, const RowsArg &vv, const int32_t *seq_ids,
-                                              const int32_t *pos, int64_t row0, int64_t n_rows, int h, uint8_t *lds) {
+                                              const int32_t *pos, int64_t row0, int64_t end, int h, uint8_t *lds) {
     constexpr int LH = HD / 16, kRowsWave = 64 / LH;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, e = lane % LH, tid = threadIdx.x;
-    const int m = (int)min((int64_t)64, n_rows - row0);
+    const int m = (int)(end - row0);
     const int t0 = pos[row0], s0 = seq_ids ? seq_ids[row0] : 0;
     bool run = t0 >= 0 && (int64_t)t0 + m <= (int64_t)g.pps * g.pt && s0 >= 0 && s0 < g.n_seq_view;
     if (tid < m) run = run && (int64_t)pos[row0 + tid] == (int64_t)t0 + tid && (!seq_ids || seq_ids[row0 + tid] == s0);
@@ -469,13 +461,15 @@ __device__ __forceinline__ void values_turned(const Geo &g, const qwfn_kv_view &
     }
     if (!run) return;
     __syncthreads();
-    // word k of a dimension: cells t0 - a + 4 k .. + 3, which lie in one tile
+    // word k of a dimension: cells t0 - a + 4 k .. + 3, which lie in one tile; the rows lie in one
+    // page or two
+    const int tb = (t0 / g.pt + 1) * g.pt;                // the second page's first cell
+    const int32_t pa = phys_page(g, v.page_table, s0, t0), pb = t0 + m > tb ? phys_page(g, v.page_table, s0, tb) : -1;
+    uint8_t *va = (uint8_t *)v.v_pages + (int64_t)pa * g.page_bytes, *vb = (uint8_t *)v.v_pages + (int64_t)pb * g.page_bytes;
     for (int i = tid; i < HD * 17; i += 256) {
         const int dim = i / 17, k = i % 17, c0 = 4 * k - a, t = t0 + c0;
-        if (c0 >= m) continue;
-        const int32_t pp = phys_page(g, v.page_table, s0, t);
-        if (pp < 0) continue;
-        uint8_t *to = (uint8_t *)v.v_pages + (int64_t)pp * g.page_bytes + vquant_off(g, h, t % g.pt, dim);
+        if (c0 >= m || (t < tb ? pa : pb) < 0) continue;
+        uint8_t *to = t < tb ? va + vquant_off(g, h, t - tb + g.pt, dim) : vb + vquant_off(g, h, t - tb, dim);
         const uint32_t w = *reinterpret_cast<const uint32_t *>(lds + dim * kTurnRow + 4 * k);
         if (c0 >= 0 && c0 + 4 <= m) {
             *reinterpret_cast<uint32_t *>(to) = w;
@@ -486,34 +480,49 @@ __device__ __forceinline__ void values_turned(const Geo &g, const qwfn_kv_view &
     }
 }
 
-// Q, K and V of 64 rows: grid (ceil(rows / 64), groups of query heads, then of key heads, then
-// one a value head).
-template <int HD, int KT, bool IL>
-__global__ void __launch_bounds__(256)
+// Q, K and V: grid (row blocks, a pass of the four waves each; groups of hq query heads, then of
+// hk key heads, then one a value head).  SZ: bytes of a source value.
+template <int HD, int KT, bool IL, int SZ>
+__global__ void __launch_bounds__(256, 3)
 k_rope_append8(Geo g, qwfn_kv_view v, RopeArg rp, RowsArg q, RowsArg k, RowsArg vv, const float *q_norm,
-               const float *k_norm, const int32_t *seq_ids, const int32_t *pos, int64_t n_rows, int n_q, RowsArg q_out) {
+               const float *k_norm, const int32_t *seq_ids, const int32_t *pos, int64_t n_rows, int n_q, int hq, int hk,
+               RowsArg q_out) {
     constexpr int kRowsWave = 64 * 16 / HD;
     __shared__ __attribute__((aligned(16))) uint8_t lds[KT == QWFN_KV_Q8_0 ? HD * kTurnRow : 16];
-    const int qg = (n_q + kHeadGroup - 1) / kHeadGroup, kg = (g.Hkv + kKeyGroup - 1) / kKeyGroup;
-    const int64_t b0 = (int64_t)blockIdx.x * 64, b1 = min(b0 + 64, n_rows);
-    const int role = blockIdx.y;
-    if (KT == QWFN_KV_Q8_0 && role >= qg + kg && g.vdim) {
-        values_turned<HD>(g, v, vv, seq_ids, pos, b0, n_rows, role - qg - kg, lds);
-        return;
+    const int qg = (n_q + hq - 1) / hq, kg = (g.Hkv + hk - 1) / hk;
+    const int64_t b0 = (int64_t)blockIdx.x * (4 * kRowsWave);
+    const int role = blockIdx.y, which = role < qg ? 0 : role < qg + kg ? 1 : 2;         // Q, K, V
+    if (KT == QWFN_KV_Q8_0 && which == 2 && g.vdim) {
+        if (b0 % 64 == 0) values_turned<HD>(g, v, vv, seq_ids, pos, b0, min(b0 + 64, n_rows), role - qg - kg, lds);
+        return;                                                                          // (64 rows a workgroup)
     }
-    for (int64_t r = b0 + (threadIdx.x >> 6) * kRowsWave; r < b1; r += 4 * kRowsWave) {
-        if (role < qg) {
-            const int h0 = role * kHeadGroup, h1 = min(h0 + kHeadGroup, n_q);
-            if (q_norm) rope_heads8<HD, IL, true>(rp, q, q_norm, pos, r, n_rows, h0, h1, q_out);
-            else rope_heads8<HD, IL, false>(rp, q, nullptr, pos, r, n_rows, h0, h1, q_out);
-        } else if (role < qg + kg) {
-            const int h0 = (role - qg) * kKeyGroup, h1 = min(h0 + kKeyGroup, g.Hkv);
-            if (k_norm) keys8<HD, IL, true, KT>(g, v, rp, k, k_norm, seq_ids, pos, r, n_rows, h0, h1);
-            else keys8<HD, IL, false, KT>(g, v, rp, k, nullptr, seq_ids, pos, r, n_rows, h0, h1);
-        } else {
-            values8<HD, KT>(g, v, vv, seq_ids, pos, r, n_rows, role - qg - kg);
+    const RowsArg src = which == 0 ? q : which == 1 ? k : vv;
+    const float *norm = which == 0 ? q_norm : which == 1 ? k_norm : nullptr;
+    const int h0 = which == 0 ? role * hq : which == 1 ? (role - qg) * hk : role - qg - kg;
+    const int h1 = which == 0 ? min(h0 + hq, n_q) : which == 1 ? min(h0 + hk, g.Hkv) : h0 + 1;
+    const int lane = threadIdx.x & 63;
+    const Place<HD, IL> pl(lane, which == 2 ? 0 : rp.rd);                                // (V does not turn)
+    const int64_t row0 = b0 + (threadIdx.x >> 6) * kRowsWave;
+    if (row0 >= n_rows) return;
+    const int64_t r = row0 + lane / pl.LH, rr = min(r, n_rows - 1);
+    const int t = pos[rr];
+    Dest d{0, 0};
+    bool live = r < n_rows;
+    if (which) {
+        const bool report = live && which == 1 && h0 == 0 && pl.e == 0;
+        live = dest_of(g, v, seq_ids ? seq_ids[rr] : 0, t, report, d) && live;
+    }
+    uint8_t *page = (uint8_t *)(which == 1 ? v.k_pages : v.v_pages) + (live ? (int64_t)d.page * g.page_bytes : 0);
+    heads8<HD, IL, SZ>(rp, pl, src, norm, rr, t, h0, h1, [&](int h, const float *x) {
+        if (which) {
+            store_chunk<KT>(g, page, h, d.row, pl.a, x, live);
+            store_chunk<KT>(g, page, h, d.row, pl.b, x + 8, live);
+        } else if (live) {
+            const int64_t to = rr * q_out.row_stride + h * q_out.head_stride;
+            store8(q_out.data, q_out.dtype, to + 8 * pl.a, x);
+            store8(q_out.data, q_out.dtype, to + 8 * pl.b, x + 8);
         }
-    }
+    });
 }
 
 // Rows that begin, every one, at a 16-byte boundary.
@@ -526,22 +535,36 @@ static bool pieces_fit(const RopeArg &rp, int hd) {
     return (hd == 64 || hd == 128 || hd == 256) && rp.rd % (rp.interleaved ? 8 : 16) == 0;
 }
 
+// Heads a wave takes with one cos and sin: four, or one while that leaves the grid under four
+// workgroups a CU (each head is then a wave's own latency; measured below).
+static int heads_a_wave(int blocks, int heads) { return (int64_t)blocks * ((heads + 3) / 4) < 1024 ? 1 : 4; }
+// Rows up to which the append takes the queries in its own launch.  Past them the launch is a few
+// per cent and the queries' kernel alone holds a wave more a SIMD.
+constexpr int kFewRows = 256;
+
+template <class F>
+static hipError_t by_shape(int hd, int dtype, F of) {
+    const auto sz = [&](auto hdc) {
+        return dtype == QWFN_SRC_F32 ? of(hdc, std::integral_constant<int, 4>()) : of(hdc, std::integral_constant<int, 2>());
+    };
+    return hd == 64 ? sz(std::integral_constant<int, 64>()) : hd == 128 ? sz(std::integral_constant<int, 128>())
+                                                                       : sz(std::integral_constant<int, 256>());
+}
+
 hipError_t launch_rope_rows(const RopeArg &rp, const RowsArg &src, const float *norm, const int32_t *pos,
                             int32_t n_rows, int32_t heads, int32_t hd, const RowsArg &dst, hipStream_t st) {
     if (pieces_fit(rp, hd) && pieces(src) && pieces(dst) && (!norm || (uintptr_t)norm % 16 == 0)) {
+        const int rows = 4 * 64 * 16 / hd, blocks = (n_rows + rows - 1) / rows, hg = heads_a_wave(blocks, heads);
         const auto go = [&](auto kern) {
-            const int rows = 4 * 64 * 16 / hd;
-            hipLaunchKernelGGL(kern, dim3((unsigned)((n_rows + rows - 1) / rows), (unsigned)((heads + kHeadGroup - 1) / kHeadGroup)),
-                               dim3(256), 0, st, rp, src, norm, pos, n_rows, heads, dst);
+            hipLaunchKernelGGL(kern, dim3((unsigned)blocks, (unsigned)((heads + hg - 1) / hg)), dim3(256), 0, st, rp, src,
+                               norm, pos, n_rows, heads, hg, dst);
             return hipGetLastError();
         };
-        const auto of = [&](auto hdc) {
-            constexpr int HD = decltype(hdc)::value;
-            if (rp.interleaved) return norm ? go(k_rope_rows8<HD, true, true>) : go(k_rope_rows8<HD, true, false>);
-            return norm ? go(k_rope_rows8<HD, false, true>) : go(k_rope_rows8<HD, false, false>);
+        const auto of = [&](auto hdc, auto szc) {
+            constexpr int HD = decltype(hdc)::value, SZ = decltype(szc)::value;
+            return rp.interleaved ? go(k_rope_rows8<HD, true, SZ>) : go(k_rope_rows8<HD, false, SZ>);
         };
-        return hd == 64 ? of(std::integral_constant<int, 64>()) : hd == 128 ? of(std::integral_constant<int, 128>())
-                                                                            : of(std::integral_constant<int, 256>());
+        return by_shape(hd, src.dtype, of);
     }
     const int64_t items = (int64_t)n_rows * heads;
     hipLaunchKernelGGL(k_rope_rows, dim3((unsigned)((items + kWaves - 1) / kWaves)), dim3(64 * kWaves), 0, st, rp, src,
@@ -557,24 +580,31 @@ hipError_t launch_rope_append(const Geo &g, const qwfn_kv_view &v, const RopeArg
     // quantized blocks of 32 are a quad of lanes' chunks: whole, when half the rotated values are
     const bool quads = g.kt == QWFN_KV_F16 || rp.interleaved || rp.rd % 64 == 0;
     const auto whole = [](const float *w) { return (uintptr_t)w % 16 == 0; };
-    if (quads && pieces_fit(rp, g.hd) && pieces(k) && pieces(vv) && (!n_q || (pieces(q) && pieces(q_out))) && whole(q_norm) &&
+    const auto size = [](const RowsArg &r) { return r.dtype == QWFN_SRC_F32 ? 4 : 2; };
+    if (quads && pieces_fit(rp, g.hd) && pieces(k) && pieces(vv) && (!n_q || (pieces(q) && pieces(q_out) && size(q) == size(k))) && size(k) == size(vv) && whole(q_norm) &&
         whole(k_norm)) {
-        const unsigned roles = (n_q + kHeadGroup - 1) / kHeadGroup + (g.Hkv + kKeyGroup - 1) / kKeyGroup + g.Hkv;
+        if (n_q && n_rows > kFewRows) {                   // the queries in a launch of their own
+            const hipError_t e = launch_rope_rows(rp, q, q_norm, pos, n_rows, n_q, g.hd, q_out, st);
+            return e != hipSuccess ? e : launch_rope_append(g, v, rp, RowsArg{}, k, vv, nullptr, k_norm, seq_ids, pos, n_rows,
+                                                            RowsArg{}, st);
+        }
+        const int rows = 4 * 64 * 16 / g.hd, blocks = (n_rows + rows - 1) / rows;
+        const int hq = heads_a_wave(blocks, std::max(n_q, 1)), hk = std::min(heads_a_wave(blocks, g.Hkv), 2);
+        const unsigned roles = (n_q + hq - 1) / hq + (g.Hkv + hk - 1) / hk + g.Hkv;
         const auto go = [&](auto kern) {
-            hipLaunchKernelGGL(kern, dim3((unsigned)(((int64_t)n_rows + 63) / 64), roles), dim3(256), 0, st, g, v, rp, q, k,
-                               vv, q_norm, k_norm, seq_ids, pos, n_rows, n_q, q_out);
+            hipLaunchKernelGGL(kern, dim3((unsigned)blocks, roles), dim3(256), 0, st, g, v, rp, q, k, vv, q_norm, k_norm,
+                               seq_ids, pos, n_rows, n_q, hq, hk, q_out);
             return hipGetLastError();
         };
-        const auto of = [&](auto hdc) {
-            constexpr int HD = decltype(hdc)::value;
+        const auto of = [&](auto hdc, auto szc) {
+            constexpr int HD = decltype(hdc)::value, SZ = decltype(szc)::value;
             if (g.kt == QWFN_KV_Q4_0)
-                return rp.interleaved ? go(k_rope_append8<HD, QWFN_KV_Q4_0, true>) : go(k_rope_append8<HD, QWFN_KV_Q4_0, false>);
+                return rp.interleaved ? go(k_rope_append8<HD, QWFN_KV_Q4_0, true, SZ>) : go(k_rope_append8<HD, QWFN_KV_Q4_0, false, SZ>);
             if (g.kt == QWFN_KV_F16)
-                return rp.interleaved ? go(k_rope_append8<HD, QWFN_KV_F16, true>) : go(k_rope_append8<HD, QWFN_KV_F16, false>);
-            return rp.interleaved ? go(k_rope_append8<HD, QWFN_KV_Q8_0, true>) : go(k_rope_append8<HD, QWFN_KV_Q8_0, false>);
+                return rp.interleaved ? go(k_rope_append8<HD, QWFN_KV_F16, true, SZ>) : go(k_rope_append8<HD, QWFN_KV_F16, false, SZ>);
+            return rp.interleaved ? go(k_rope_append8<HD, QWFN_KV_Q8_0, true, SZ>) : go(k_rope_append8<HD, QWFN_KV_Q8_0, false, SZ>);
         };
-        return g.hd == 64 ? of(std::integral_constant<int, 64>()) : g.hd == 128 ? of(std::integral_constant<int, 128>())
-                                                                                : of(std::integral_constant<int, 256>());
+        return by_shape(g.hd, k.dtype, of);
     }
     const int64_t items = (int64_t)n_rows * (n_q + 2 * g.Hkv);
     hipLaunchKernelGGL(k_rope_append, dim3((unsigned)((items + kWaves - 1) / kWaves)), dim3(64 * kWaves), 0, st, g, v,
