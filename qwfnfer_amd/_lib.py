@@ -162,7 +162,6 @@ _V = C.POINTER(KvView)
 _IS = C.POINTER(IdxShape)
 _IV = C.POINTER(IdxView)
 _R = C.POINTER(RopeStruct)
-_RW = C.POINTER(RowsStruct)
 _P = C.c_void_p
 _I = C.c_int32
 _Z = C.c_size_t
@@ -205,8 +204,8 @@ _SIGS = {
                                               _P, _Z, _P]),
     "qwfn_idx_sparse_attn_prefill": (C.c_int, [_S, _V, _IS, _IV, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P,
                                                _I, _P, _Z, _P]),
-    "qwfn_rope_rows": (C.c_int, [_R, _RW, _P, _P, _I, _I, _I, _I, _RW, _P]),
-    "qwfn_kv_append_rope": (C.c_int, [_S, _V, _R, _RW, _RW, _P, _P, _P, _I, _RW, _P, _RW, _P]),
+    "qwfn_rope_rows": (C.c_int, [_R, _P, _P, _P, _I, _I, _I, _I, _P, _P]),
+    "qwfn_kv_append_rope": (C.c_int, [_S, _V, _R, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P]),
     "qwfn_window_workspace_bytes": (C.c_int, [_S, _I, _I, _I, _I, _I, _I, _I, C.POINTER(_Z)]),
     "qwfn_window_attn_decode": (C.c_int, [_S, _V, _P, _I, _P, _I, _I, _I, _I, _P, _P, _Z, _P]),
     "qwfn_window_attn_prefill": (C.c_int, [_S, _V, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _Z, _P]),

@@ -535,9 +535,15 @@ static bool pieces_fit(const RopeArg &rp, int hd) {
     return (hd == 64 || hd == 128 || hd == 256) && rp.rd % (rp.interleaved ? 8 : 16) == 0;
 }
 
-// Heads a wave takes with one cos and sin: four, or one while that leaves the grid under four
-// workgroups a CU (each head is then a wave's own latency; measured below).
-static int heads_a_wave(int blocks, int heads) { return (int64_t)blocks * ((heads + 3) / 4) < 1024 ? 1 : 4; }
+// Heads a wave takes with one cos and sin: the fewest of 1, 2 and 4 that leave the grid within
+// the 1,024 workgroups resident at once, else 4 (cos and sin are a fourth of a wave's
+// instructions at 4 heads and more than half at 1; fewer heads a wave fill the device with few
+// rows: 64 rows of 20 heads 5.7 us with 1, 14 with 4).
+static int heads_a_wave(int blocks, int heads) {
+    for (int n = 1; n < 4; n *= 2)
+        if ((int64_t)blocks * ((heads + n - 1) / n) <= 1024) return n;
+    return 4;
+}
 // Rows up to which the append takes the queries in its own launch.  Past them the launch is a few
 // per cent and the queries' kernel alone holds a wave more a SIMD.
 constexpr int kFewRows = 256;

@@ -16,13 +16,14 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence
 
 import torch
 
 from . import _lib
-from ._lib import IdxShape, IdxView, KvView, QsaShape, RopeStruct, RowsStruct, call
+from ._lib import IdxShape, IdxView, KvView, QsaShape, RopeStruct, call
 
 __all__ = [
     "QsaConfig", "KvCache", "KvState", "Workspace",
@@ -917,34 +918,45 @@ class Rope:
         self._c = RopeStruct(cfg.rope_dim, _lib.ROPE_HALF if cfg.layout == "half" else _lib.ROPE_INTERLEAVED,
                              self.turns.data_ptr(), cfg.scale(), cfg.norm_eps)
 
-    def c_struct(self) -> RopeStruct:
-        return self._c
+    def c_ref(self):
+        return C.byref(self._c)
 
 
-def _rows(t: torch.Tensor, name: str, n_rows: int, n_heads: int, head_dim: int, device: torch.device) -> RowsStruct:
-    """Head rows [n_rows, n_heads, head_dim] with any row and head stride."""
+_pack_rows = struct.Struct("@Piqq").pack                  # qwfn_rows
+
+
+def _rows(t: torch.Tensor, name: str, n_rows: int, n_heads: int, head_dim: int, device: int) -> bytes:
+    """The C struct of head rows [n_rows, n_heads, head_dim] with any row and head stride, on a device."""
+    # the usual case in one expression; what fails it is told apart below (a struct packed into bytes
+    # and the device by its number: 1 us a tensor less than a ctypes struct and torch.device)
+    if isinstance(t, torch.Tensor) and t.shape == (n_rows, n_heads, head_dim) and t.get_device() == device and device >= 0:
+        dtype = _DTYPES.get(t.dtype)
+        rs, hs, one = t.stride()
+        if dtype is not None and (one == 1 or head_dim == 1):
+            return _pack_rows(t.data_ptr(), dtype, rs, hs)
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    dtype = _dtype(t.dtype, name)
-    if t.device != device or device.type != "cuda":
-        raise ValueError(f"{name} must be on the device of the other tensors, {device}; it is on {t.device}")
+    _dtype(t.dtype, name)
+    if not t.is_cuda or t.get_device() != device:
+        raise ValueError(f"{name} must be on the device of the other tensors; it is on {t.device}")
     if tuple(t.shape) != (n_rows, n_heads, head_dim):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {(n_rows, n_heads, head_dim)}")
-    rs, hs, one = t.stride()
-    if one != 1 and head_dim > 1:
-        raise ValueError(f"{name}: the values of a head row must be contiguous")
-    return RowsStruct(t.data_ptr(), dtype, rs, hs)
+    raise ValueError(f"{name}: the values of a head row must be contiguous")
 
 
-def _beside(device: torch.device, **tensors) -> None:
+def _beside(device: int, **tensors) -> None:
     for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} must be on {device}, it is on {t.device}")
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"{name} must be on device {device}, it is on {t.device}")
 
 
-def _call_on(device: torch.device, stream, name: str, *args) -> None:
+def _call_on(device: int, stream, name: str, *args) -> None:
     """An entry point on the tensors' device, whichever is the current one."""
-    if device.index == torch.cuda.current_device():
+    try:                                             # (not part of torch's public interface)
+        current = torch._C._cuda_getDevice()
+    except AttributeError:
+        current = torch.cuda.current_device()
+    if device == current:
         call(name, *args, _stream(stream))
         return
     with torch.cuda.device(device):
@@ -963,9 +975,9 @@ def rope_rows(rope: Rope, x: torch.Tensor, pos: torch.Tensor, norm: Optional[tor
     if not isinstance(x, torch.Tensor) or x.dim() != 3:
         raise ValueError("x must be a tensor [n_rows, n_heads, head_dim]")
     n, heads, hd = x.shape
-    dev = x.device
+    dev = x.get_device()
     if out is None:
-        out = torch.empty((n, heads, hd), dtype=x.dtype, device=dev)
+        out = torch.empty((n, heads, hd), dtype=x.dtype, device=x.device)
     if n == 0:                                       # no rows: nothing to launch
         return out
     src, dst = _rows(x, "x", n, heads, hd, dev), _rows(out, "out", n, heads, hd, dev)
@@ -973,8 +985,8 @@ def rope_rows(rope: Rope, x: torch.Tensor, pos: torch.Tensor, norm: Optional[tor
     if norm is not None:
         _need(norm, "norm", torch.float32, hd)
     _beside(dev, pos=pos, norm=norm, turns=rope.turns)
-    _call_on(dev, stream, "qwfn_rope_rows", C.byref(rope.c_struct()), C.byref(src), _ptr(norm), pos.data_ptr(), n,
-             heads, hd, 1 if inverse else 0, C.byref(dst))
+    _call_on(dev, stream, "qwfn_rope_rows", rope.c_ref(), src, _ptr(norm), pos.data_ptr(), n, heads, hd,
+             1 if inverse else 0, dst)
     return out
 
 
@@ -990,34 +1002,35 @@ def append_rope(cache: KvCache, rope: Rope, k: torch.Tensor, v: torch.Tensor, po
     head_dim], those are normed (``q_norm``) and turned in the same launch into
     ``q_out`` (default float32), which is returned."""
     cfg = cache.cfg
-    n, dev = pos.numel(), cache.k_pages.device
+    n, dev = pos.numel(), cache.k_pages.get_device()
     if q is None and (q_norm is not None or q_out is not None):
         raise ValueError("q_norm and q_out come with q")
     if q is not None and q_out is None:
-        q_out = torch.empty((n, cfg.n_head, cfg.head_dim), dtype=torch.float32, device=dev)
+        q_out = torch.empty((n, cfg.n_head, cfg.head_dim), dtype=torch.float32, device=cache.k_pages.device)
     if n == 0:
         return q_out
-    kr, vr = (_rows(t, m, n, cfg.n_head_kv, cfg.head_dim, dev) for t, m in ((k, "k"), (v, "v")))
+    hkv, hd = cfg.n_head_kv, cfg.head_dim
+    kr, vr = _rows(k, "k", n, hkv, hd, dev), _rows(v, "v", n, hkv, hd, dev)
     qr = qo = None
     if q is not None:
-        qr, qo = (_rows(t, m, n, cfg.n_head, cfg.head_dim, dev) for t, m in ((q, "q"), (q_out, "q_out")))
+        qr, qo = _rows(q, "q", n, cfg.n_head, hd, dev), _rows(q_out, "q_out", n, cfg.n_head, hd, dev)
     _need(pos, "pos", torch.int32, n)
     if seq_ids is not None:
         _need(seq_ids, "seq_ids", torch.int32, n)
-    for t, m in ((k_norm, "k_norm"), (q_norm, "q_norm")):
-        if t is not None:
-            _need(t, m, torch.float32, cfg.head_dim)
+    if k_norm is not None:
+        _need(k_norm, "k_norm", torch.float32, hd)
+    if q_norm is not None:
+        _need(q_norm, "q_norm", torch.float32, hd)
     _beside(dev, pos=pos, seq_ids=seq_ids, k_norm=k_norm, q_norm=q_norm, turns=rope.turns)
-    _call_on(dev, stream, "qwfn_kv_append_rope", C.byref(cache.c_shape()), C.byref(cache.view()),
-             C.byref(rope.c_struct()), C.byref(kr), C.byref(vr), _ptr(k_norm), _ptr(seq_ids), pos.data_ptr(), n,
-             None if qr is None else C.byref(qr), _ptr(q_norm), None if qo is None else C.byref(qo))
+    _call_on(dev, stream, "qwfn_kv_append_rope", C.byref(cache.c_shape()), C.byref(cache.view()), rope.c_ref(),
+             kr, vr, _ptr(k_norm), _ptr(seq_ids), pos.data_ptr(), n, qr, _ptr(q_norm), qo)
     return q_out
 
 
 # ---- sliding-window attention ------------------------------------------------
 
 def _window_rows(cache: KvCache, q: torch.Tensor, n_rows: Optional[int], out: Optional[torch.Tensor], ws: Workspace):
-    cfg, dev = cache.cfg, cache.k_pages.device
+    cfg, dev = cache.cfg, cache.k_pages.get_device()
     if not isinstance(q, torch.Tensor):
         raise TypeError("q must be a torch.Tensor")
     width = cfg.n_head * cfg.head_dim
@@ -1026,7 +1039,7 @@ def _window_rows(cache: KvCache, q: torch.Tensor, n_rows: Optional[int], out: Op
     dtype = _dtype(q.dtype, "q")
     _need(q, "q", q.dtype, n_rows * width)
     if out is None:
-        out = torch.empty((n_rows, cfg.n_head, cfg.head_dim), dtype=q.dtype, device=dev)
+        out = torch.empty((n_rows, cfg.n_head, cfg.head_dim), dtype=q.dtype, device=q.device)
     _need(out, "out", q.dtype, n_rows * width)
     _beside(dev, q=q, out=out, ws=ws.buf)
     return dtype, n_rows, out, dev
