@@ -8,6 +8,8 @@
 
 namespace qwfn_qsa {
 
+constexpr int kWinMostParts = 256;       // parts a row's tiles are split into
+
 inline size_t win_align(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // The 64-cell tiles that the last n_q queries of a sequence of length len see: the

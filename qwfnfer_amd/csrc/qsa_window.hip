@@ -489,7 +489,7 @@ static PfLayout pf_layout(const Geo &g, const WinPlan &p) {
     l.blocks = (int)blocks;
     // few blocks: their tiles over several workgroups, at least two tiles each
     const int64_t wgs = blocks * g.Hkv;
-    l.parts = (int)std::max<int64_t>(1, std::min<int64_t>(l.cap / 2, 512 / wgs));
+    l.parts = (int)std::max<int64_t>(1, std::min<int64_t>({l.cap / 2, 512 / wgs, kWinMostParts}));
     size_t off = win_align((size_t)p.n_seq * g.Hkv * l.cap * (size_t)(planes(p) * 64 * g.hd * 2) * 2);
     auto take = [&](size_t bytes) { const size_t o = off; off = win_align(off + bytes); return o; };
     l.info = take((size_t)p.n_seq * g.Hkv * l.cap * sizeof(TileInfo));

@@ -189,8 +189,12 @@ k_win_dec(Geo g, qwfn_kv_view v, WinArg wa, int parts, float *part_o, float2 *pa
     if (rows != 1) {                                    // none, or too many, which get zeros
         for (int64_t i = threadIdx.x; i < (int64_t)rows * g.G; i += 256) {
             const int64_t at = row + i / g.G;
-            if (parts > 1) part_rl[((at * g.Hkv + gh) * parts + part) * g.G + i % g.G] = make_float2(-INFINITY, 0.0f);
-            else for (int d = 0; d < HD; d += 4) store4(wa.out, wa.dtype, (at * g.H + gh * g.G + i % g.G) * HD + d, f4v{0, 0, 0, 0});
+            const int64_t pr = ((at * g.Hkv + gh) * parts + part) * g.G + i % g.G;
+            if (parts > 1) part_rl[pr] = make_float2(-INFINITY, 0.0f);
+            for (int d = 0; d < HD; d += 4) {
+                if (parts > 1) *reinterpret_cast<f4v *>(part_o + pr * HD + d) = f4v{0, 0, 0, 0};
+                else store4(wa.out, wa.dtype, (at * g.H + gh * g.G + i % g.G) * HD + d, f4v{0, 0, 0, 0});
+            }
         }
         return;
     }
@@ -416,13 +420,13 @@ k_win_dec(Geo g, qwfn_kv_view v, WinArg wa, int parts, float *part_o, float2 *pa
         float ls = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float f = __builtin_amdgcn_exp2f(rl[k][h].x - ref);
-            if (rl[k][h].x == -INFINITY) continue;      // no tile: nothing of it counts
+            // (weights of 0 are multiplied all the same: a seen value that is not finite shows)
+            const float f = rl[k][h].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(rl[k][h].x - ref);
             y += f * *reinterpret_cast<const f4v *>(reinterpret_cast<const float *>(lds[k]) + at);
             ls += f * rl[k][h].y;
         }
         if (parts == 1) {
-            store4(wa.out, wa.dtype, ((int64_t)row * g.H + gh * g.G) * HD + at, ls != 0.0f ? y / ls : f4v{0, 0, 0, 0});
+            store4(wa.out, wa.dtype, ((int64_t)row * g.H + gh * g.G) * HD + at, y * (ls != 0.0f ? 1.0f / ls : 0.0f));
         } else {
             const int64_t pr = (((int64_t)row * g.Hkv + gh) * parts + part) * g.G;
             *reinterpret_cast<f4v *>(part_o + pr * HD + at) = y;
@@ -431,40 +435,120 @@ k_win_dec(Geo g, qwfn_kv_view v, WinArg wa, int parts, float *part_o, float2 *pa
     }
 }
 
-// The parts of one row and query head: grid (Hkv * G, rows), HD / 4 threads.
-__global__ void __launch_bounds__(64)
+// The parts of one row and query head, grid (rows, Hkv * G): every wave finds the weights (lane k
+// takes part k, k + 64, ...), thread (j, d) sums parts j, j + 1024 / HD, ... of values 4 d ..
+// + 3, the loads of four parts in flight, and LDS joins the j.
+template <int HD>
+__global__ void __launch_bounds__(256)
 k_win_merge(Geo g, WinArg wa, int parts, const float *part_o, const float2 *part_rl) {
-    const int h = blockIdx.x, gh = h / g.G, row = blockIdx.y, d = threadIdx.x * 4;
+    constexpr int D = HD / 4, J = 256 / D;
+    __shared__ f4v sum[256];
+    __shared__ float ws[4 * 64];                          // weights of up to kWinMostParts parts
+    const int h = blockIdx.y, gh = h / g.G, row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, d = tid % D, j = tid / D;
     if (wa.q_start && (row < wa.q_start[0] || row >= wa.q_start[wa.n_seq])) return;
     const int64_t first = ((int64_t)row * g.Hkv + gh) * parts * g.G + h % g.G;
+    float2 rl[kWinMostParts / 64];
     float rm = -INFINITY;
-    for (int k = 0; k < parts; ++k) rm = fmaxf(rm, part_rl[first + (int64_t)k * g.G].x);
+#pragma unroll
+    for (int k = 0; k < kWinMostParts / 64; ++k) {
+        const int p = 64 * k + lane;
+        rl[k] = p < parts ? part_rl[first + (int64_t)p * g.G] : make_float2(-INFINITY, 0.0f);
+        rm = fmaxf(rm, rl[k].x);
+    }
+    rm = wave_max(rm);
+    const float ref = rm == -INFINITY ? 0.0f : rm;
+    float ls = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWinMostParts / 64; ++k) {
+        const float f = rl[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(rl[k].x - ref);
+        ls += f * rl[k].y;
+        if (tid < 64) ws[64 * k + lane] = f;
+    }
+    ls = wave_sum(ls);
+    __syncthreads();
+    f4v y = {0, 0, 0, 0};
+    for (int p = j; p < parts; p += 4 * J) {
+        f4v o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int at = min(p + k * J, parts - 1);
+            o[k] = *reinterpret_cast<const f4v *>(part_o + (first + (int64_t)at * g.G) * HD + 4 * d);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (p + k * J < parts) y += ws[p + k * J] * o[k];
+    }
+    sum[tid] = y;
+    __syncthreads();
+    if (j) return;
+#pragma unroll
+    for (int k = 1; k < J; ++k) y += sum[k * D + d];
+    store4(wa.out, wa.dtype, ((int64_t)row * g.H + h) * HD + 4 * d, y * (ls != 0.0f ? 1.0f / ls : 0.0f));
+}
+
+// The same for up to kFewParts parts: a thread four values of a row and head, no exchange, the
+// rows of several workgroups' worth in one (many rows of few parts: 700 x 16 heads x 5 parts
+// 17 us by k_win_merge).
+constexpr int kFewParts = 8;
+template <int HD>
+__global__ void __launch_bounds__(256)
+k_win_merge_few(Geo g, WinArg wa, int parts, const float *part_o, const float2 *part_rl) {
+    const int64_t i = (int64_t)blockIdx.x * (1024 / HD) + threadIdx.x / (HD / 4);           // row * H + head
+    const int64_t row = i / g.H;
+    const int h = (int)(i % g.H), d = threadIdx.x % (HD / 4) * 4;
+    if (row >= wa.n_rows) return;
+    if (wa.q_start && (row < wa.q_start[0] || row >= wa.q_start[wa.n_seq])) return;
+    const int64_t first = (row * g.Hkv + h / g.G) * parts * g.G + h % g.G;
+    float2 rl[kFewParts];
+    f4v o[kFewParts];
+    float rm = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kFewParts; ++k) {
+        const int64_t at = first + (int64_t)min(k, parts - 1) * g.G;
+        rl[k] = part_rl[at];
+        o[k] = *reinterpret_cast<const f4v *>(part_o + at * HD + d);
+    }
+#pragma unroll
+    for (int k = 0; k < kFewParts; ++k) {
+        if (k >= parts) rl[k].x = -INFINITY;
+        rm = fmaxf(rm, rl[k].x);
+    }
     const float ref = rm == -INFINITY ? 0.0f : rm;
     f4v y = {0, 0, 0, 0};
     float ls = 0.0f;
-#pragma unroll 4
-    for (int k = 0; k < parts; ++k) {
-        const int64_t at = first + (int64_t)k * g.G;
-        const float2 rl = part_rl[at];
-        const f4v o = *reinterpret_cast<const f4v *>(part_o + at * g.hd + d);
-        const bool none = rl.x == -INFINITY;            // a part without a tile (its o may not be written)
-        const float f = none ? 0.0f : __builtin_amdgcn_exp2f(rl.x - ref);
-        y += none ? f4v{0, 0, 0, 0} : f * o;
-        ls += f * rl.y;
+#pragma unroll
+    for (int k = 0; k < kFewParts; ++k) {
+        if (k >= parts) break;
+        const float f = rl[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(rl[k].x - ref);
+        ls += f * rl[k].y;
+        y += f * o[k];
     }
-    store4(wa.out, wa.dtype, ((int64_t)row * g.H + h) * g.hd + d, ls != 0.0f ? y / ls : f4v{0, 0, 0, 0});
+    store4(wa.out, wa.dtype, (row * g.H + h) * HD + d, y * (ls != 0.0f ? 1.0f / ls : 0.0f));
+}
+
+template <int HD>
+static void merge_t(const Geo &g, const WinArg &wa, int parts, const float *part_o, const float2 *part_rl, hipStream_t st) {
+    if (parts <= kFewParts) {
+        const int64_t rows = (int64_t)wa.n_rows * g.H, a_wg = 1024 / HD;
+        hipLaunchKernelGGL(k_win_merge_few<HD>, dim3((unsigned)((rows + a_wg - 1) / a_wg)), dim3(256), 0, st, g, wa, parts,
+                           part_o, part_rl);
+    } else {
+        hipLaunchKernelGGL(k_win_merge<HD>, dim3((unsigned)wa.n_rows, (unsigned)g.H), dim3(256), 0, st, g, wa, parts, part_o,
+                           part_rl);
+    }
 }
 
 void launch_win_merge(const Geo &g, const WinArg &wa, int parts, const float *part_o, const float2 *part_rl, hipStream_t st) {
-    hipLaunchKernelGGL(k_win_merge, dim3((unsigned)g.H, (unsigned)wa.n_rows), dim3((unsigned)g.hd / 4), 0, st, g, wa, parts,
-                       part_o, part_rl);
+    if (g.hd == 64) merge_t<64>(g, wa, parts, part_o, part_rl, st);
+    else if (g.hd == 128) merge_t<128>(g, wa, parts, part_o, part_rl, st);
+    else merge_t<256>(g, wa, parts, part_o, part_rl, st);
 }
 
 // Parts of a sequence's tiles: enough workgroups for two a CU, at most a tile a wave.
 int win_dec_parts(const Geo &g, const WinPlan &p) {
     const int tiles = win_most_tiles(p);
     const int pairs = p.n_seq * g.Hkv;
-    return std::max(1, std::min((tiles + 3) / 4, (512 + pairs - 1) / pairs));
+    return std::max(1, std::min({(tiles + 3) / 4, (512 + pairs - 1) / pairs, kWinMostParts}));
 }
 
 size_t win_dec_ws_bytes(const Geo &g, const WinPlan &p) {
