@@ -276,25 +276,30 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int parts, const uint8_t *
     const int64_t first = ((int64_t)s * g.Hkv + gh) * cap;
     auto cell_of = [&](int k) { const int t = k / (64 / TC); return (t < n1 ? t : wt + t - n1) * 64 + k % (64 / TC) * TC; };
     auto slot_of = [&](int cell) { const int t = cell / 64; return t < tl.ns ? t : tl.ns + t - tl.w0; };
-    // one step's K and V, 16 bytes a lane, into buffer k & 1
+    // one step's K and V, 16 bytes a lane, into buffer k & 1.  The wave's transfers of 1 KiB differ
+    // by uniform offsets alone, so each costs no vector register: K [plane][chunk][TC][8] is runs of
+    // TC cells of the tile's 64, V [plane][TC / 16][2][HD][8] is one run a plane.
+    const uint32_t lane_k = lane / TC * 1024 + lane % TC * 16, lane_v = lane * 16;
     auto fetch = [&](int k) {
-        const int cell = cell_of(k);
+        const int cell = cell_of(k), sub = cell % 64;
         const uint8_t *src = staged + (first + slot_of(cell)) * (int64_t)(2 * staged_half<HD, NP>());
-        const int sub = cell % 64;
         const uint32_t dst = (uint32_t)(uintptr_t)lds + (k & 1) * kStep;
 #pragma unroll
         for (int i = 0; i < kHalf / 4096; ++i) {
             const int at = (i * 4 + w) * 1024;            // LDS bytes of the wave's transfer
-            // K [plane][chunk][TC][8]: a run of TC cells within the tile's 64
-            const int b = at + lane * 16;
-            lds_dma16_sv(src, (uint32_t)(b / (TC * 16) * 1024 + sub * 16 + b % (TC * 16)), dst + at);
+            lds_dma16_sv(src + at / (TC * 16) * 1024 + sub * 16, lane_k, dst + at);
         }
 #pragma unroll
         for (int i = 0; i < kHalf / 4096; ++i) {
-            const int at = (i * 4 + w) * 1024;
-            const int b = at + lane * 16, pl = b / (TC * HD * 2), in = b % (TC * HD * 2);
-            lds_dma16_sv(src, (uint32_t)(staged_half<HD, NP>() + pl * 64 * HD * 2 + sub * HD * 2 + in), dst + kHalf + at);
+            const int at = (i * 4 + w) * 1024, pl = at / (TC * HD * 2);
+            lds_dma16_sv(src + staged_half<HD, NP>() + pl * (64 - TC) * HD * 2 + sub * HD * 2 + at, lane_v, dst + kHalf + at);
         }
+    };
+    // (through the scalar cache: a vector load would wait for the transfers issued before it)
+    auto info_of = [&](int k) {
+        typedef const __attribute__((address_space(4))) int32_t *Const;
+        const Const p = (Const)(uintptr_t)(info + first + slot_of(cell_of(k)));
+        return TileInfo{p[0], p[1], p[2], p[3]};
     };
 
     f16v o[RB][DT];
@@ -312,13 +317,18 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int parts, const uint8_t *
     // the wave's own range of positions, for the masks
     const int64_t rw = min(r0 + (int64_t)w * RB * 32, total - 1);
     const int pw_lo = base + (int)(rw / g.G), pw_hi = base + (int)(min(r0 + (int64_t)(w + 1) * RB * 32 - 1, total - 1) / g.G);
-    if (k0 < k1) fetch(k0);
+    TileInfo next{0, 0, 0, 0};
+    if (k0 < k1) {
+        fetch(k0);
+        next = info_of(k0);
+    }
     for (int k = k0; k < k1; ++k) {
         wait_vmem_all();
         __syncthreads();
         if (k + 1 < k1) fetch(k + 1);
         const int t0 = cell_of(k);
-        const TileInfo ti = info[first + slot_of(t0)];
+        const TileInfo ti = next;
+        if (k + 1 < k1) next = info_of(k + 1);
         if (!ti.there) continue;
         const uint8_t *kb = lds + (k & 1) * kStep, *vb = kb + kHalf;
         if (ti.ve != ve) {                                // V in other units from here on
