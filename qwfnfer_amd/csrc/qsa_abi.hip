@@ -1298,7 +1298,7 @@ int qwfn_window_workspace_bytes(const qwfn_qsa_shape *shape, int32_t n_seq, int3
 }
 
 static int window_attn(const char *what, const qwfn_qsa_shape *shape, const qwfn_kv_view *view, const WinPlan &p,
-                       const WinArg &wa, void *ws, size_t ws_bytes, void *stream) {
+                       WinArg wa, void *ws, size_t ws_bytes, void *stream) {
     Geo g;
     int rc = make_geo(shape, view, &g);
     if (rc) return rc;
@@ -1317,6 +1317,9 @@ static int window_attn(const char *what, const qwfn_qsa_shape *shape, const qwfn
     if (!ws || !aligned(ws, 256)) return fail(QWFN_EINVAL, "%s: workspace NULL or not 256-byte aligned", what);
     const size_t need = window_ws_bytes(g, p);
     if (ws_bytes < need) return fail(QWFN_ERANGE, "%s: workspace of %zu bytes < %zu needed", what, ws_bytes, need);
+    // (past every position they say the same, and the kernels' differences stay within 32 bits)
+    wa.window = std::min(wa.window, p.max_seq_len);
+    wa.sinks = std::min(wa.sinks, p.max_seq_len);
     const hipError_t e = launch_window(g, *view, wa, p, ws, (hipStream_t)stream);
     return e == hipSuccess ? ok() : hip_fail(e, what);
 }

@@ -30,17 +30,19 @@ namespace {
 //   K [plane][hd / 8][64 cells][8 dims]
 //   V [plane][64 / 16][2][hd][8 cells]: cells 16 ks + 4 half + {0 .. 3, 8 .. 11}
 template <int HD, int NP> constexpr int staged_half() { return NP * 64 * HD * 2; }     // bytes of K, or of V
-// What the rows' kernel needs to know of it: values are staged times 2^ke, 2^ve.
+// What the rows' kernel needs to know of a tile: values are staged times 2^ke, 2^ve.
 struct TileInfo {
     int32_t ke, ve;
     int32_t there;          // the tile's page is in the pool
-    int32_t odd;            // V holds values that are not finite
+    int32_t odd;            // V holds values that are not finite: staged as 0, their bits in OddBits
 };
+// Where an odd tile's V is not finite: bit d % 32 of word [cell][d / 32].
+template <int HD> constexpr int odd_words() { return 64 * HD / 32; }
 
 // A plan's staging area: tiles [n_seq][Hkv][cap], their TileInfo, then the parts.
 struct PfLayout {
     int cap, parts, blocks;
-    size_t info, part_o, part_rl, total;
+    size_t info, odd, part_o, part_rl, total;
 };
 
 constexpr int kExact = 2;   // planes of float32 and float16 rows
@@ -57,6 +59,15 @@ __device__ __forceinline__ PfSeq pf_seq(const WinArg &wa, int s) {
     return q;
 }
 
+// Whether the query at pos sees cell t0 + c: c against three numbers, so that a lane holds no
+// cell indices.
+struct Seen {
+    int last, before, sinks;
+    __device__ __forceinline__ Seen(int pos, int window, int sink_tokens, int t0)
+        : last(pos - t0), before(pos - window - t0), sinks(sink_tokens - t0) {}
+    __device__ __forceinline__ bool operator()(int c) const { return c <= last && (c > before || c < sinks); }
+};
+
 // e with |x| 2^e < 2^15 for |x| <= m, in steps, so that neighbouring tiles mostly share it
 // (a change costs the rows' kernel a pass over its sums).  fp16's absolute half step 2^-25 is
 // then small against the tile's largest value: one plane, 0 while m is in [2^-4, 2^15), so
@@ -72,7 +83,8 @@ __device__ __forceinline__ int stage_exp(float m) {
 // grid (tile slots, Hkv, n_seq): slot i of a sequence's list of tiles into its place.
 template <int HD, int KT, bool VD, int NP>
 __global__ void __launch_bounds__(256)
-k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo *info) {
+k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo *info,
+            uint32_t *odd_bits) {
     constexpr int NB = HD / 32, C8 = HD / 8, kRow = HD + 8;
     __shared__ float dk[64][NB + 1], dv[64][NB + 1];
     __shared__ float red[2][4];
@@ -149,8 +161,14 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
     // plane p of a value: its fp16, or what the fp16 leaves
     auto plane = [&](float x, int p) {
         const _Float16 h = (_Float16)x;
-        if (p == 0) return h;
-        return fabsf(x) < INFINITY ? (_Float16)(x - (float)h) : (_Float16)0.0f;
+        return p == 0 ? h : (_Float16)(x - (float)h);
+    };
+    int odd = 0;
+    // a V value, 0 in place of one that is not finite: a row that does not see it multiplies it by 0
+    auto finite = [&](float x) {
+        const bool fin = fabsf(x) < INFINITY;
+        odd |= !fin;
+        return fin ? x : 0.0f;
     };
     for (int i = tid; i < C8 * 64; i += 256) {
         float x[8];
@@ -164,7 +182,6 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
         }
     }
     out += staged_half<HD, NP>();
-    int odd = 0;
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
         if constexpr (!VD) {
@@ -174,10 +191,7 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
                 eight(vq, dv, i >> 6, i & 63, fv, x);
                 h8v y;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    y[k] = plane(x[k], p);
-                    odd |= !(fabsf((float)y[k]) < INFINITY);
-                }
+                for (int k = 0; k < 8; ++k) y[k] = plane(finite(x[k]), p);
                 *reinterpret_cast<h8v *>(&vt[i & 63][(i >> 6) * 8]) = y;
             }
             __syncthreads();
@@ -191,8 +205,7 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const int cell = c0 + (k < 4 ? k : k + 4);
-                    y[k] = plane(dv[cell][dim / 32] * fv * (float)(int8_t)((k < 4 ? a : b) >> (8 * (k & 3))), p);
-                    odd |= !(fabsf((float)y[k]) < INFINITY);
+                    y[k] = plane(finite(dv[cell][dim / 32] * fv * (float)(int8_t)((k < 4 ? a : b) >> (8 * (k & 3)))), p);
                 }
             } else {
 #pragma unroll
@@ -202,6 +215,14 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
         }
     }
     odd = __syncthreads_or(odd);
+    if (odd)
+        for (int i = tid; i < odd_words<HD>(); i += 256) {
+            uint32_t bits = 0;
+            for (int d = 0; d < 32; ++d)
+                bits |= (uint32_t)(i / NB < live && !(fabsf(member_k(g, (const uint8_t *)v.v_pages + (int64_t)pp * g.page_bytes, gh,
+                                                                     t0 % g.pt + i / NB, i % NB * 32 + d, true)) < INFINITY)) << d;
+            odd_bits[at * odd_words<HD>() + i] = bits;
+        }
     if (tid == 0) info[at] = TileInfo{ke, ve, 1, odd};
 }
 
@@ -209,8 +230,8 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
 // the KV head's group.  TC cells a step, double-buffered in LDS.
 template <int HD, int NP, int TC, int RB>
 __global__ void __launch_bounds__(256, HD == 256 || RB == 2 ? 1 : 2)
-k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int parts, const uint8_t *staged, const TileInfo *info, float *part_o,
-           float2 *part_rl) {
+k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int parts, const uint8_t *staged, const TileInfo *info,
+           const uint32_t *odd_bits, float *part_o, float2 *part_rl) {
     constexpr int KS = HD / 16, DT = HD / 32, CT = TC / 32, kRows = 128 * RB;
     constexpr int kHalf = NP * TC * HD * 2, kStep = 2 * kHalf;            // bytes of K (or V), of both
     constexpr float kOff = NP == 2 ? 13.0f : 6.0f, kSlack = NP == 2 ? 2.0f : 8.0f;
@@ -313,7 +334,7 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int parts, const uint8_t *
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[b][d][i] = 0.0f;
     }
-    int ve = 0;
+    int ve = 0, any_odd = 0;
     // the wave's own range of positions, for the masks
     const int64_t rw = min(r0 + (int64_t)w * RB * 32, total - 1);
     const int pw_lo = base + (int)(rw / g.G), pw_hi = base + (int)(min(r0 + (int64_t)(w + 1) * RB * 32 - 1, total - 1) / g.G);
@@ -369,14 +390,12 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int parts, const uint8_t *
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
             if (!whole) {
-                const int lo = pos[b] - wa.window;
+                const Seen see(pos[b], wa.window, wa.sinks, t0 + 4 * half);
 #pragma unroll
                 for (int c = 0; c < CT; ++c)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int t = t0 + c * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-                        x[b][c][i] = t <= pos[b] && (t > lo || t < wa.sinks) ? x[b][c][i] : -INFINITY;
-                    }
+                    for (int i = 0; i < 16; ++i)
+                        x[b][c][i] = see(c * 32 + 8 * (i >> 2) + (i & 3)) ? x[b][c][i] : -INFINITY;
             }
             float mx = x[b][0][0];
 #pragma unroll
@@ -404,63 +423,45 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int parts, const uint8_t *
                 }
         }
         // ---- O^T ----
-        if (!ti.odd || whole) {
+        any_odd |= ti.odd;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int ks = 0; ks < TC / 16; ++ks) {
-                    h8v a[NP];
+            for (int ks = 0; ks < TC / 16; ++ks) {
+                h8v a[NP];
 #pragma unroll
-                    for (int p = 0; p < NP; ++p)
-                        a[p] = *reinterpret_cast<const h8v *>(vb + p * (TC * HD * 2) + ((2 * ks + half) * HD + 32 * d + n) * 16);
-#pragma unroll
-                    for (int b = 0; b < RB; ++b) {
-                        if constexpr (NP == 2) {
-                            o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], pf[0][b][ks], o[b][d], 0, 0, 0);
-                            o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[1][b][ks], o[b][d], 0, 0, 0);
-                        }
-                        o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[0][b][ks], o[b][d], 0, 0, 0);
-                    }
-                }
-        } else {
-            // values that are not finite, which some row does not see: they are left out of the
-            // products, and a row that does see one gets a NaN there
-#pragma unroll 1
-            for (int d = 0; d < DT; ++d)
+                for (int p = 0; p < NP; ++p)
+                    a[p] = *reinterpret_cast<const h8v *>(vb + p * (TC * HD * 2) + ((2 * ks + half) * HD + 32 * d + n) * 16);
 #pragma unroll
                 for (int b = 0; b < RB; ++b) {
-                    f16v cnt, add;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) cnt[i] = add[i] = 0.0f;
-#pragma unroll
-                    for (int ks = 0; ks < TC / 16; ++ks) {
-                        const int lo = pos[b] - wa.window;
-                        h8v a[NP], bad, vis;
-#pragma unroll
-                        for (int p = 0; p < NP; ++p)
-                            a[p] = *reinterpret_cast<const h8v *>(vb + p * (TC * HD * 2) + ((2 * ks + half) * HD + 32 * d + n) * 16);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int t = t0 + 16 * ks + 8 * (i >> 2) + 4 * half + (i & 3);
-                            const bool fin = fabsf((float)a[0][i]) < INFINITY;
-                            bad[i] = fin ? (_Float16)0.0f : (_Float16)1.0f;
-                            vis[i] = t <= pos[b] && (t > lo || t < wa.sinks) ? (_Float16)1.0f : (_Float16)0.0f;
-                            a[0][i] = fin ? a[0][i] : (_Float16)0.0f;
-                        }
-                        cnt = __builtin_amdgcn_mfma_f32_32x32x16_f16(bad, vis, cnt, 0, 0, 0);
-                        add = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[0][b][ks], add, 0, 0, 0);
-                        if constexpr (NP == 2) {
-                            add = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], pf[0][b][ks], add, 0, 0, 0);
-                            add = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[1][b][ks], add, 0, 0, 0);
-                        }
+                    if constexpr (NP == 2) {
+                        o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], pf[0][b][ks], o[b][d], 0, 0, 0);
+                        o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[1][b][ks], o[b][d], 0, 0, 0);
                     }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) add[i] = cnt[i] > 0.0f ? NAN : add[i];
-#pragma unroll
-                    for (int dd = 0; dd < DT; ++dd)       // (registers are not indexed by a loop's variable)
-                        if (dd == d) o[b][dd] += add;
+                    o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[0][b][ks], o[b][d], 0, 0, 0);
                 }
-        }
+            }
+    }
+    // ---- values that are not finite: a row that sees one gets a NaN there ----
+    for (int k = k0; any_odd && k < k1; ++k) {
+        const TileInfo ti = info_of(k);
+        if (!ti.there || !ti.odd) continue;
+        const int t0 = cell_of(k);
+        const uint32_t *bits = odd_bits + (first + slot_of(t0)) * odd_words<HD>() + t0 % 64 * DT;
+#pragma unroll 1
+        for (int c = 0; c < TC; ++c)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const uint32_t m = bits[c * DT + d] >> (4 * half);
+                if (m == 0) continue;
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    const bool see = Seen(pos[b], wa.window, wa.sinks, t0)(c);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        o[b][d][i] = see && (m >> (8 * (i >> 2) + (i & 3)) & 1) ? NAN : o[b][d][i];
+                }
+            }
     }
 
     // ---- out ----
@@ -503,6 +504,7 @@ static PfLayout pf_layout(const Geo &g, const WinPlan &p) {
     size_t off = win_align((size_t)p.n_seq * g.Hkv * l.cap * (size_t)(planes(p) * 64 * g.hd * 2) * 2);
     auto take = [&](size_t bytes) { const size_t o = off; off = win_align(off + bytes); return o; };
     l.info = take((size_t)p.n_seq * g.Hkv * l.cap * sizeof(TileInfo));
+    l.odd = take((size_t)p.n_seq * g.Hkv * l.cap * (64 * g.hd / 32) * sizeof(uint32_t));
     const size_t pr = l.parts > 1 ? (size_t)p.n_rows * g.Hkv * l.parts * g.G : 0;
     l.part_o = take(pr * g.hd * sizeof(float));
     l.part_rl = take(pr * sizeof(float2));
@@ -513,7 +515,7 @@ static PfLayout pf_layout(const Geo &g, const WinPlan &p) {
 template <int HD, int KT, bool VD, int NP>
 static void stage_t(const Geo &g, const qwfn_kv_view &v, const WinArg &wa, const PfLayout &l, uint8_t *ws, hipStream_t st) {
     hipLaunchKernelGGL((k_win_stage<HD, KT, VD, NP>), dim3((unsigned)l.cap, (unsigned)g.Hkv, (unsigned)wa.n_seq), dim3(256),
-                       0, st, g, v, wa, l.cap, ws, (TileInfo *)(ws + l.info));
+                       0, st, g, v, wa, l.cap, ws, (TileInfo *)(ws + l.info), (uint32_t *)(ws + l.odd));
 }
 
 template <int HD, int NP, int TC, int RB>
@@ -527,7 +529,7 @@ static hipError_t prefill_t(const Geo &g, const qwfn_kv_view &v, const WinArg &w
                                              hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((k_win_rows<HD, NP, TC, RB>), dim3((unsigned)(l.blocks * l.parts), (unsigned)g.Hkv), dim3(256), kLds,
-                       st, g, v, wa, l.cap, l.parts, ws, (const TileInfo *)(ws + l.info), (float *)(ws + l.part_o),
+                       st, g, v, wa, l.cap, l.parts, ws, (const TileInfo *)(ws + l.info), (const uint32_t *)(ws + l.odd), (float *)(ws + l.part_o),
                        (float2 *)(ws + l.part_rl));
     if (l.parts > 1) launch_win_merge(g, wa, l.parts, (const float *)(ws + l.part_o), (const float2 *)(ws + l.part_rl), st);
     return hipGetLastError();
