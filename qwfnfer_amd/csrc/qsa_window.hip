@@ -45,6 +45,7 @@ struct PfLayout {
     size_t info, odd, part_o, part_rl, total;
 };
 
+constexpr int kEighths = 1024;   // workgroups from which neighbouring blocks share an XCD (340 against 351 us at 1,024)
 constexpr int kExact = 2;   // planes of float32 and float16 rows
 
 // The sequence's queries and length, and whether they can be served.
@@ -226,18 +227,29 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
     if (tid == 0) info[at] = TileInfo{ke, ve, 1, odd};
 }
 
-// grid (row blocks * parts, Hkv), four waves of 32 RB rows each; row = query * G + head of
-// the KV head's group.  TC cells a step, double-buffered in LDS.
+// Four waves of 32 RB rows each; row = query * G + head of the KV head's group.  TC cells a
+// step, double-buffered in LDS.  One-dimensional grid over blocks * parts * Hkv: a workgroup's
+// XCD is its index modulo 8, and each XCD takes a run of neighbouring blocks of one KV head,
+// whose windows overlap and fit its L2 (4 MB).
 template <int HD, int NP, int TC, int RB>
 __global__ void __launch_bounds__(256, HD == 256 || RB == 2 ? 1 : 2)
-k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int parts, const uint8_t *staged, const TileInfo *info,
+k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int blocks, int parts, const uint8_t *staged, const TileInfo *info,
            const uint32_t *odd_bits, float *part_o, float2 *part_rl) {
     constexpr int KS = HD / 16, DT = HD / 32, CT = TC / 32, kRows = 128 * RB;
     constexpr int kHalf = NP * TC * HD * 2, kStep = 2 * kHalf;            // bytes of K (or V), of both
     constexpr float kOff = NP == 2 ? 13.0f : 6.0f, kSlack = NP == 2 ? 2.0f : 8.0f;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n = lane & 31, half = lane >> 5, gh = blockIdx.y, part = blockIdx.x % parts, blk = blockIdx.x / parts;
+    const int n = lane & 31, half = lane >> 5;
+    // the blocks of one sequence's worth of rows, in eighths when they are more than the device
+    // holds at once, then one more a sequence
+    const int full = blocks - wa.n_seq, n_full = full * parts * g.Hkv;
+    int id = (int)blockIdx.x;
+    const bool tail = id >= n_full;
+    if (tail) id -= n_full;
+    else if (n_full >= kEighths && id < n_full / 8 * 8) id = id % 8 * (n_full / 8) + id / 8;
+    const int per = tail ? wa.n_seq : full;
+    const int gh = id / (per * parts), part = id % parts, blk = id / parts % per + (tail ? full : 0);
     // the block's sequence: blocks of sequence s start at q_start[s] * G / kRows + s
     int s = 0;
     for (int hi = wa.n_seq - 1; s < hi;) {
@@ -528,8 +540,7 @@ static hipError_t prefill_t(const Geo &g, const qwfn_kv_view &v, const WinArg &w
     const hipError_t e = hipFuncSetAttribute((const void *)k_win_rows<HD, NP, TC, RB>,
                                              hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((k_win_rows<HD, NP, TC, RB>), dim3((unsigned)(l.blocks * l.parts), (unsigned)g.Hkv), dim3(256), kLds,
-                       st, g, v, wa, l.cap, l.parts, ws, (const TileInfo *)(ws + l.info), (const uint32_t *)(ws + l.odd), (float *)(ws + l.part_o),
+    hipLaunchKernelGGL((k_win_rows<HD, NP, TC, RB>), dim3((unsigned)(l.blocks * l.parts * g.Hkv)), dim3(256), kLds, st, g, v, wa, l.cap, l.blocks, l.parts, ws, (const TileInfo *)(ws + l.info), (const uint32_t *)(ws + l.odd), (float *)(ws + l.part_o),
                        (float2 *)(ws + l.part_rl));
     if (l.parts > 1) launch_win_merge(g, wa, l.parts, (const float *)(ws + l.part_o), (const float2 *)(ws + l.part_rl), st);
     return hipGetLastError();
