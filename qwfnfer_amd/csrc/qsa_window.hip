@@ -227,15 +227,15 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
     if (tid == 0) info[at] = TileInfo{ke, ve, 1, odd};
 }
 
-// Four waves of 32 RB rows each; row = query * G + head of the KV head's group.  TC cells a
+// Four waves of 32 rows each; row = query * G + head of the KV head's group.  TC cells a
 // step, double-buffered in LDS.  One-dimensional grid over blocks * parts * Hkv: a workgroup's
 // XCD is its index modulo 8, and each XCD takes a run of neighbouring blocks of one KV head,
 // whose windows overlap and fit its L2 (4 MB).
-template <int HD, int NP, int TC, int RB>
-__global__ void __launch_bounds__(256, HD == 256 || RB == 2 ? 1 : 2)
+template <int HD, int NP, int TC>
+__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
 k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int blocks, int parts, const uint8_t *staged, const TileInfo *info,
            const uint32_t *odd_bits, float *part_o, float2 *part_rl) {
-    constexpr int KS = HD / 16, DT = HD / 32, CT = TC / 32, kRows = 128 * RB;
+    constexpr int KS = HD / 16, DT = HD / 32, CT = TC / 32, kRows = 128;
     constexpr int kHalf = NP * TC * HD * 2, kStep = 2 * kHalf;            // bytes of K (or V), of both
     constexpr float kOff = NP == 2 ? 13.0f : 6.0f, kSlack = NP == 2 ? 2.0f : 8.0f;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -263,21 +263,18 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int blocks, int parts, con
     const int base = q.len - q.n_q;                       // position of the sequence's first query
 
     // ---- the rows' queries ----
-    h8v qf[NP][RB][KS];
-    float c0[RB];
-    int pos[RB];
-    int64_t io[RB];                                       // the row's first value, -1: none
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        const int64_t rr = r0 + (w * RB + b) * 32 + n;
-        const int qi = (int)(rr / g.G), h = gh * g.G + (int)(rr % g.G);
-        io[b] = rr < total ? (((int64_t)q.start + qi) * g.H + h) * HD : -1;
-        pos[b] = base + (rr < total ? qi : q.n_q - 1);
+    h8v qf[NP][KS];
+    const int64_t rr = r0 + w * 32 + n;
+    const bool row = rr < total;
+    const int qi = (int)(rr / g.G), pos = base + (row ? qi : q.n_q - 1);
+    const int64_t io = (((int64_t)q.start + qi) * g.H + gh * g.G + (int)(rr % g.G)) * HD;     // the row's first value
+    float c0;
+    {
         float x[KS][8], m = 0.0f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            if (io[b] >= 0) {
-                load8(wa.q, wa.dtype, io[b] + 16 * k + 8 * half, x[k]);
+            if (row) {
+                load8(wa.q, wa.dtype, io + 16 * k + 8 * half, x[k]);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[k][j] = 0.0f;
@@ -285,17 +282,16 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int blocks, int parts, con
 #pragma unroll
             for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[k][j]));
         }
-        m = swap32_op(m, [](float a, float c) { return fmaxf(a, c); });
-        const int e = pow2_to(m, 13);
+        const int e = pow2_to(swap32_op(m, [](float a, float c) { return fmaxf(a, c); }), 13);
         const float f = ldexpf(1.0f, e);
-        c0[b] = ldexpf(g.scale_log2, -e);
+        c0 = ldexpf(g.scale_log2, -e);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float y = x[k][j] * f;
-                qf[0][b][k][j] = (_Float16)y;
-                if constexpr (NP == 2) qf[NP - 1][b][k][j] = (_Float16)(y - (float)(_Float16)y);
+                qf[0][k][j] = (_Float16)y;
+                if constexpr (NP == 2) qf[NP - 1][k][j] = (_Float16)(y - (float)(_Float16)y);
             }
     }
 
@@ -335,21 +331,17 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int blocks, int parts, con
         return TileInfo{p[0], p[1], p[2], p[3]};
     };
 
-    f16v o[RB][DT];
-    float r[RB], l[RB];
+    f16v o[DT];
+    float r = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        r[b] = -INFINITY;
-        l[b] = 0.0f;
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[b][d][i] = 0.0f;
-    }
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     int ve = 0, any_odd = 0;
     // the wave's own range of positions, for the masks
-    const int64_t rw = min(r0 + (int64_t)w * RB * 32, total - 1);
-    const int pw_lo = base + (int)(rw / g.G), pw_hi = base + (int)(min(r0 + (int64_t)(w + 1) * RB * 32 - 1, total - 1) / g.G);
+    const int64_t rw = min(r0 + w * 32, total - 1);
+    const int pw_lo = base + (int)(rw / g.G), pw_hi = base + (int)(min(r0 + w * 32 + 31, total - 1) / g.G);
+
     TileInfo next{0, 0, 0, 0};
     if (k0 < k1) {
         fetch(k0);
@@ -363,79 +355,72 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int blocks, int parts, con
         const TileInfo ti = next;
         if (k + 1 < k1) next = info_of(k + 1);
         if (!ti.there) continue;
+        any_odd |= ti.odd;
         const uint8_t *kb = lds + (k & 1) * kStep, *vb = kb + kHalf;
         if (ti.ve != ve) {                                // V in other units from here on
             const float f = ldexpf(1.0f, ti.ve - ve);
             ve = ti.ve;
 #pragma unroll
-            for (int b = 0; b < RB; ++b)
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[b][d] *= f;
+            for (int d = 0; d < DT; ++d) o[d] *= f;
         }
-        // ---- S^T ----
-        f16v x[RB][CT];
+        // ---- S^T; the matrix halves go before the other wave's vector half (340 -> 322 us) ----
+        __builtin_amdgcn_s_setprio(1);
+        f16v x[CT];
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
 #pragma unroll
-            for (int b = 0; b < RB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[b][c][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) x[c][i] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 h8v a[NP];
 #pragma unroll
                 for (int p = 0; p < NP; ++p)
                     a[p] = *reinterpret_cast<const h8v *>(kb + p * (TC * HD * 2) + ((2 * ks + half) * TC + c * 32 + n) * 16);
-#pragma unroll
-                for (int b = 0; b < RB; ++b) {
-                    if constexpr (NP == 2) {
-                        x[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], qf[0][b][ks], x[b][c], 0, 0, 0);
-                        x[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], qf[1][b][ks], x[b][c], 0, 0, 0);
-                    }
-                    x[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], qf[0][b][ks], x[b][c], 0, 0, 0);
+                if constexpr (NP == 2) {
+                    x[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], qf[0][ks], x[c], 0, 0, 0);
+                    x[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], qf[1][ks], x[c], 0, 0, 0);
                 }
+                x[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], qf[0][ks], x[c], 0, 0, 0);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         // ---- masks, the running reference, the weights ----
         const bool whole = t0 + TC - 1 <= pw_lo && (t0 > pw_hi - wa.window || t0 + TC <= wa.sinks);
-        h8v pf[NP][RB][CT * 2];
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-            if (!whole) {
-                const Seen see(pos[b], wa.window, wa.sinks, t0 + 4 * half);
-#pragma unroll
-                for (int c = 0; c < CT; ++c)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        x[b][c][i] = see(c * 32 + 8 * (i >> 2) + (i & 3)) ? x[b][c][i] : -INFINITY;
-            }
-            float mx = x[b][0][0];
+        if (!whole) {
+            const Seen see(pos, wa.window, wa.sinks, t0 + 4 * half);
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[b][c][i]);
-            mx = swap32_op(mx, [](float p, float q2) { return fmaxf(p, q2); });
-            const float cs = ldexpf(c0[b], -ti.ke), want = mx * cs - kOff;
-            if (__any(want > r[b] + kSlack)) {
-                const float rn = fmaxf(r[b], want), f = __builtin_amdgcn_exp2f(r[b] - (rn == -INFINITY ? 0.0f : rn));
-                r[b] = rn;
-                l[b] *= f;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[b][d] *= f;
-            }
-            const float ref = r[b] == -INFINITY ? 0.0f : r[b];
-#pragma unroll
-            for (int c = 0; c < CT; ++c)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(fmaf(x[b][c][i], cs, -ref));
-                    l[b] += e;
-                    pf[0][b][2 * c + (i >> 3)][i & 7] = (_Float16)e;
-                    if constexpr (NP == 2) pf[NP - 1][b][2 * c + (i >> 3)][i & 7] = (_Float16)(e - (float)(_Float16)e);
-                }
+                for (int i = 0; i < 16; ++i)
+                    x[c][i] = see(c * 32 + 8 * (i >> 2) + (i & 3)) ? x[c][i] : -INFINITY;
         }
+        float mx = x[0][0];
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[c][i]);
+        mx = swap32_op(mx, [](float p, float q2) { return fmaxf(p, q2); });
+        const float cs = ldexpf(c0, -ti.ke), want = mx * cs - kOff;
+        if (__any(want > r + kSlack)) {
+            const float rn = fmaxf(r, want), f = __builtin_amdgcn_exp2f(r - (rn == -INFINITY ? 0.0f : rn));
+            r = rn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] *= f;
+        }
+        const float ref = r == -INFINITY ? 0.0f : r;
+        h8v pf[NP][CT * 2];
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(x[c][i], cs, -ref));
+                l += e;
+                pf[0][2 * c + (i >> 3)][i & 7] = (_Float16)e;
+                if constexpr (NP == 2) pf[NP - 1][2 * c + (i >> 3)][i & 7] = (_Float16)(e - (float)(_Float16)e);
+            }
         // ---- O^T ----
-        any_odd |= ti.odd;
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -444,15 +429,13 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int blocks, int parts, con
 #pragma unroll
                 for (int p = 0; p < NP; ++p)
                     a[p] = *reinterpret_cast<const h8v *>(vb + p * (TC * HD * 2) + ((2 * ks + half) * HD + 32 * d + n) * 16);
-#pragma unroll
-                for (int b = 0; b < RB; ++b) {
-                    if constexpr (NP == 2) {
-                        o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], pf[0][b][ks], o[b][d], 0, 0, 0);
-                        o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[1][b][ks], o[b][d], 0, 0, 0);
-                    }
-                    o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[0][b][ks], o[b][d], 0, 0, 0);
+                if constexpr (NP == 2) {
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], pf[0][ks], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[1][ks], o[d], 0, 0, 0);
                 }
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[0][ks], o[d], 0, 0, 0);
             }
+        __builtin_amdgcn_s_setprio(0);
     }
     // ---- values that are not finite: a row that sees one gets a NaN there ----
     for (int k = k0; any_odd && k < k1; ++k) {
@@ -466,35 +449,28 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int blocks, int parts, con
             for (int d = 0; d < DT; ++d) {
                 const uint32_t m = bits[c * DT + d] >> (4 * half);
                 if (m == 0) continue;
+                const bool see = Seen(pos, wa.window, wa.sinks, t0)(c);
 #pragma unroll
-                for (int b = 0; b < RB; ++b) {
-                    const bool see = Seen(pos[b], wa.window, wa.sinks, t0)(c);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        o[b][d][i] = see && (m >> (8 * (i >> 2) + (i & 3)) & 1) ? NAN : o[b][d][i];
-                }
+                for (int i = 0; i < 16; ++i) o[d][i] = see && (m >> (8 * (i >> 2) + (i & 3)) & 1) ? NAN : o[d][i];
             }
     }
 
     // ---- out ----
+    const float ls = swap32_op(l, [](float p, float q2) { return p + q2; });
+    if (!row) return;
+    const float f = ldexpf(1.0f, -ve) * (parts == 1 ? (ls != 0.0f ? 1.0f / ls : 0.0f) : 1.0f);
+    const int64_t pr = ((((int64_t)q.start + qi) * g.Hkv + gh) * parts + part) * g.G + rr % g.G;
+    if (parts > 1 && half == 0) part_rl[pr] = make_float2(r, ls);
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        const float ls = swap32_op(l[b], [](float p, float q2) { return p + q2; });
-        if (io[b] < 0) continue;
-        const float f = ldexpf(1.0f, -ve) * (parts == 1 ? (ls != 0.0f ? 1.0f / ls : 0.0f) : 1.0f);
-        const int64_t row = io[b] / HD, pr = ((row / g.H * g.Hkv + gh) * parts + part) * g.G + row % g.G;
-        if (parts > 1 && half == 0) part_rl[pr] = make_float2(r[b], ls);
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f4v y = {o[b][d][4 * i], o[b][d][4 * i + 1], o[b][d][4 * i + 2], o[b][d][4 * i + 3]};
-                y *= f;
-                const int at = 32 * d + 8 * i + 4 * half;
-                if (parts > 1) *reinterpret_cast<f4v *>(part_o + pr * HD + at) = y;
-                else store4(wa.out, wa.dtype, io[b] + at, y);
-            }
-    }
+        for (int i = 0; i < 4; ++i) {
+            f4v y = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+            y *= f;
+            const int at = 32 * d + 8 * i + 4 * half;
+            if (parts > 1) *reinterpret_cast<f4v *>(part_o + pr * HD + at) = y;
+            else store4(wa.out, wa.dtype, io + at, y);
+        }
 }
 
 // ---------------------------------------------------------------------------
@@ -530,17 +506,17 @@ static void stage_t(const Geo &g, const qwfn_kv_view &v, const WinArg &wa, const
                        0, st, g, v, wa, l.cap, ws, (TileInfo *)(ws + l.info), (uint32_t *)(ws + l.odd));
 }
 
-template <int HD, int NP, int TC, int RB>
+template <int HD, int NP, int TC>
 static hipError_t prefill_t(const Geo &g, const qwfn_kv_view &v, const WinArg &wa, const PfLayout &l, uint8_t *ws, hipStream_t st) {
     if (g.kt == QWFN_KV_Q4_0) stage_t<HD, QWFN_KV_Q4_0, false, NP>(g, v, wa, l, ws, st);
     else if (g.kt == QWFN_KV_F16) stage_t<HD, QWFN_KV_F16, false, NP>(g, v, wa, l, ws, st);
     else if (g.vdim) stage_t<HD, QWFN_KV_Q8_0, true, NP>(g, v, wa, l, ws, st);
     else stage_t<HD, QWFN_KV_Q8_0, false, NP>(g, v, wa, l, ws, st);
     constexpr int kLds = 2 * 2 * NP * TC * HD * 2;
-    const hipError_t e = hipFuncSetAttribute((const void *)k_win_rows<HD, NP, TC, RB>,
+    const hipError_t e = hipFuncSetAttribute((const void *)k_win_rows<HD, NP, TC>,
                                              hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((k_win_rows<HD, NP, TC, RB>), dim3((unsigned)(l.blocks * l.parts * g.Hkv)), dim3(256), kLds, st, g, v, wa, l.cap, l.blocks, l.parts, ws, (const TileInfo *)(ws + l.info), (const uint32_t *)(ws + l.odd), (float *)(ws + l.part_o),
+    hipLaunchKernelGGL((k_win_rows<HD, NP, TC>), dim3((unsigned)(l.blocks * l.parts * g.Hkv)), dim3(256), kLds, st, g, v, wa, l.cap, l.blocks, l.parts, ws, (const TileInfo *)(ws + l.info), (const uint32_t *)(ws + l.odd), (float *)(ws + l.part_o),
                        (float2 *)(ws + l.part_rl));
     if (l.parts > 1) launch_win_merge(g, wa, l.parts, (const float *)(ws + l.part_o), (const float2 *)(ws + l.part_rl), st);
     return hipGetLastError();
@@ -558,9 +534,9 @@ hipError_t launch_window(const Geo &g, const qwfn_kv_view &v, const WinArg &wa, 
     uint8_t *b = (uint8_t *)ws;
     const bool exact = planes(p) == kExact;
     switch (g.hd) {
-    case 64: return exact ? prefill_t<64, 2, 64, 1>(g, v, wa, l, b, st) : prefill_t<64, 1, 64, 1>(g, v, wa, l, b, st);
-    case 128: return exact ? prefill_t<128, 2, 32, 1>(g, v, wa, l, b, st) : prefill_t<128, 1, 64, 1>(g, v, wa, l, b, st);
-    case 256: return exact ? prefill_t<256, 2, 32, 1>(g, v, wa, l, b, st) : prefill_t<256, 1, 32, 1>(g, v, wa, l, b, st);
+    case 64: return exact ? prefill_t<64, 2, 64>(g, v, wa, l, b, st) : prefill_t<64, 1, 64>(g, v, wa, l, b, st);
+    case 128: return exact ? prefill_t<128, 2, 32>(g, v, wa, l, b, st) : prefill_t<128, 1, 64>(g, v, wa, l, b, st);
+    case 256: return exact ? prefill_t<256, 2, 32>(g, v, wa, l, b, st) : prefill_t<256, 1, 32>(g, v, wa, l, b, st);
     }
     return hipErrorInvalidValue;
 }
