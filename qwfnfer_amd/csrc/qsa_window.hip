@@ -17,6 +17,8 @@
 //     order) the operand layout of P^T, so weights never leave their lane.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "qsa_append.h"
 #include "qsa_window.h"
 
@@ -112,6 +114,30 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
     const int64_t tile = (int64_t)pp * g.page_bytes + (int64_t)(gh * (g.pt / 64) + t0 % g.pt / 64) * g.chunks * 1024;
     const uint8_t *kq = (const uint8_t *)v.k_pages + tile, *vq = (const uint8_t *)v.v_pages + tile;
     const int live = q.len - t0;                          // cells of the tile that are written
+    // ---- every piece the thread converts, in flight before the scales are waited for ----
+    // item i of K (and of V in a K layout): dims 8 (i / 64) .. of cell i % 64; of a dimension-major V: cells
+    // c0 .. c0 + 3 and c0 + 8 .. c0 + 11 of dim i % HD
+    constexpr int N = HD / 32;                            // items a thread: tid + 256 n
+    using Piece = std::conditional_t<KT == QWFN_KV_F16, u4v, uint2>;
+    Piece kr[N], vr[N];
+    auto piece = [&](const uint8_t *tq, int i) {
+        const int c8 = i >> 6, cell = i & 63;
+        if constexpr (KT == QWFN_KV_F16) return *reinterpret_cast<const u4v *>(tq + c8 * 1024 + cell * 16);
+        else if constexpr (KT == QWFN_KV_Q4_0) return *reinterpret_cast<const uint2 *>(tq + (c8 / 4) * 1024 + cell * 16 + (c8 & 1) * 8);
+        else return *reinterpret_cast<const uint2 *>(tq + (c8 / 2) * 1024 + cell * 16 + (c8 & 1) * 8);
+    };
+    auto cell0 = [](int i) { return i / HD / 2 * 16 + (i / HD & 1) * 4; };
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int i = tid + 256 * n;
+        kr[n] = piece(kq, i);
+        if constexpr (VD) {
+            const uint8_t *p = vq + i % HD * 64 + cell0(i);
+            vr[n] = make_uint2(*reinterpret_cast<const uint32_t *>(p), *reinterpret_cast<const uint32_t *>(p + 8));
+        } else {
+            vr[n] = piece(vq, i);
+        }
+    }
     // ---- the scales, and the exponents they ask for ----
     int ke = 0, ve = 0;
     if constexpr (KT != QWFN_KV_F16) {
@@ -136,10 +162,10 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
     }
     const float fk = ldexpf(1.0f, ke), fv = ldexpf(1.0f, ve);
     uint8_t *out = staged + at * (2 * staged_half<HD, NP>());
-    // eight values (8 dims of one cell) of a K-layout tile, times the exponent's power of two
-    auto eight = [&](const uint8_t *tq, const float (*d)[NB + 1], int c8, int cell, float f, float *x) {
+    // the eight values of a K-layout piece, times the exponent's power of two
+    auto eight = [&](Piece w, const float (*d)[NB + 1], int i, float f, float *x) {
+        const int c8 = i >> 6, cell = i & 63;
         if constexpr (KT == QWFN_KV_F16) {
-            const u4v w = *reinterpret_cast<const u4v *>(tq + c8 * 1024 + cell * 16);
 #pragma unroll
             for (int k = 0; k < 4; ++k) { x[2 * k] = h2f((uint16_t)w[k]); x[2 * k + 1] = h2f((uint16_t)(w[k] >> 16)); }
             if (cell >= live)
@@ -147,15 +173,11 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
                 for (int k = 0; k < 8; ++k) x[k] = 0.0f;
         } else {
             const float dd = d[cell][c8 / 4] * f;
-            if constexpr (KT == QWFN_KV_Q4_0) {
-                const uint2 w = *reinterpret_cast<const uint2 *>(tq + (c8 / 4) * 1024 + cell * 16 + (c8 & 1) * 8);
-                const int sh = c8 & 2 ? 4 : 0;
+            const int sh = c8 & 2 ? 4 : 0;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = dd * (float)((int)((k < 4 ? w.x : w.y) >> (8 * (k & 3) + sh) & 15) - 8);
-            } else {
-                const uint2 w = *reinterpret_cast<const uint2 *>(tq + (c8 / 2) * 1024 + cell * 16 + (c8 & 1) * 8);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = dd * (float)(int8_t)((k < 4 ? w.x : w.y) >> (8 * (k & 3)));
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t u = (k < 4 ? w.x : w.y) >> (8 * (k & 3));
+                x[k] = dd * (KT == QWFN_KV_Q4_0 ? (float)((int)(u >> sh & 15) - 8) : (float)(int8_t)u);
             }
         }
     };
@@ -171,9 +193,11 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
         odd |= !fin;
         return fin ? x : 0.0f;
     };
-    for (int i = tid; i < C8 * 64; i += 256) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int i = tid + 256 * n;
         float x[8];
-        eight(kq, dk, i >> 6, i & 63, fk, x);
+        eight(kr[n], dk, i, fk, x);
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
             h8v y;
@@ -187,9 +211,11 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
     for (int p = 0; p < NP; ++p) {
         if constexpr (!VD) {
             __syncthreads();
-            for (int i = tid; i < C8 * 64; i += 256) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int i = tid + 256 * n;
                 float x[8];
-                eight(vq, dv, i >> 6, i & 63, fv, x);
+                eight(vr[n], dv, i, fv, x);
                 h8v y;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) y[k] = plane(finite(x[k]), p);
@@ -197,16 +223,15 @@ k_win_stage(Geo g, qwfn_kv_view v, WinArg wa, int cap, uint8_t *staged, TileInfo
             }
             __syncthreads();
         }
-        for (int i = tid; i < HD * 8; i += 256) {         // i = (ks * 2 + half) * HD + dim
-            const int dim = i % HD, c0 = i / HD / 2 * 16 + (i / HD & 1) * 4;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = tid + 256 * n, dim = i % HD, c0 = cell0(i);           // i = (ks * 2 + half) * HD + dim
             h8v y;
             if constexpr (VD) {
-                const uint32_t a = *reinterpret_cast<const uint32_t *>(vq + dim * 64 + c0);
-                const uint32_t b = *reinterpret_cast<const uint32_t *>(vq + dim * 64 + c0 + 8);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const int cell = c0 + (k < 4 ? k : k + 4);
-                    y[k] = plane(finite(dv[cell][dim / 32] * fv * (float)(int8_t)((k < 4 ? a : b) >> (8 * (k & 3)))), p);
+                    y[k] = plane(finite(dv[cell][dim / 32] * fv * (float)(int8_t)((k < 4 ? vr[n].x : vr[n].y) >> (8 * (k & 3)))), p);
                 }
             } else {
 #pragma unroll
