@@ -71,6 +71,20 @@ struct Seen {
     __device__ __forceinline__ bool operator()(int c) const { return c <= last && (c > before || c < sinks); }
 };
 
+// The order of a run of N products whose operand (NP planes) comes from LDS: reads kAhead
+// products ahead.  Left to itself the compiler reads each operand where it is used, and its LDS
+// latency (some 130 cycles) shows between the products.
+template <int NP, int N>
+__device__ __forceinline__ void lds_ahead() {
+    constexpr int kAhead = N < 4 ? N : 4;
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead * NP, 0);                    // LDS reads
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NP == 2 ? 3 : 1, 0);            // MFMA
+        if (i + kAhead < N) __builtin_amdgcn_sched_group_barrier(0x100, NP, 0);
+    }
+}
+
 // e with |x| 2^e < 2^15 for |x| <= m, in steps, so that neighbouring tiles mostly share it
 // (a change costs the rows' kernel a pass over its sums).  fp16's absolute half step 2^-25 is
 // then small against the tile's largest value: one plane, 0 while m is in [2^-4, 2^15), so
@@ -266,15 +280,20 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int blocks, int parts, con
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, half = lane >> 5;
-    // the blocks of one sequence's worth of rows, in eighths when they are more than the device
-    // holds at once, then one more a sequence
-    const int full = blocks - wa.n_seq, n_full = full * parts * g.Hkv;
-    int id = (int)blockIdx.x;
-    const bool tail = id >= n_full;
-    if (tail) id -= n_full;
-    else if (n_full >= kEighths && id < n_full / 8 * 8) id = id % 8 * (n_full / 8) + id / 8;
-    const int per = tail ? wa.n_seq : full;
-    const int gh = id / (per * parts), part = id % parts, blk = id / parts % per + (tail ? full : 0);
+    // one more block a sequence than whole ones.  More than the device holds at once: each XCD an
+    // eighth of them, by heads and rows.  Fewer: the last rows of all heads first, as the first
+    // ones see less (a compute unit's second workgroup is then a short one: 102 -> 90 us at 3,001
+    // float32 queries from nothing)
+    int id = (int)blockIdx.x, gh, part, blk;
+    if (blocks * parts * g.Hkv >= kEighths) {
+        const int full = blocks - wa.n_seq, n_full = full * parts * g.Hkv, tail = id >= n_full;
+        if (tail) id -= n_full;
+        else if (id < n_full / 8 * 8) id = id % 8 * (n_full / 8) + id / 8;
+        const int per = tail ? wa.n_seq : full;
+        gh = id / (per * parts), part = id % parts, blk = id / parts % per + (tail ? full : 0);
+    } else {
+        gh = id % g.Hkv, part = id / g.Hkv % parts, blk = blocks - 1 - id / (g.Hkv * parts);
+    }
     // the block's sequence: blocks of sequence s start at q_start[s] * G / kRows + s
     int s = 0;
     for (int hi = wa.n_seq - 1; s < hi;) {
@@ -408,6 +427,7 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int blocks, int parts, con
                 x[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], qf[0][ks], x[c], 0, 0, 0);
             }
         }
+        lds_ahead<NP, CT * KS>();
         __builtin_amdgcn_s_setprio(0);
         // ---- masks, the running reference, the weights ----
         const bool whole = t0 + TC - 1 <= pw_lo && (t0 > pw_hi - wa.window || t0 + TC <= wa.sinks);
@@ -460,6 +480,7 @@ k_win_rows(Geo g, qwfn_kv_view v, WinArg wa, int cap, int blocks, int parts, con
                 }
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], pf[0][ks], o[d], 0, 0, 0);
             }
+        lds_ahead<NP, DT * TC / 16>();
         __builtin_amdgcn_s_setprio(0);
     }
     // ---- values that are not finite: a row that sees one gets a NaN there ----
