@@ -155,13 +155,17 @@ struct Place {
 // A lane's cos and sin: IL: of chunk a's four pairs and b's; HALF: of the eight pairs of a and b.
 template <int HD, bool IL>
 __device__ __forceinline__ void place_cs(const Place<HD, IL> &pl, const RopeArg &rp, int pos, double2 (&cs)[8]) {
-    double p = (double)pos;
+    double p = (double)pos, f[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {                         // (every load before the first is used)
+        const bool on = k < 4 || !IL ? pl.ta : pl.tb;
+        f[k] = rp.turns[on ? IL ? 4 * (k < 4 ? pl.a : pl.b) + (k & 3) : 8 * pl.a + k : 0];
+    }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         cs[k] = make_double2(0.0, 0.0);
         if (k < 4 || !IL ? pl.ta : pl.tb) {
-            const int i = IL ? 4 * (k < 4 ? pl.a : pl.b) + (k & 3) : 8 * pl.a + k;
-            const double2 t = turn(p, rp.turns[i]);
+            const double2 t = turn(p, f[k]);
             cs[k] = make_double2(t.x * rp.mscale, (rp.inverse ? -t.y : t.y) * rp.mscale);
         }
         // one pair after the other: eight chains at once would take the registers of a wave more a SIMD
@@ -419,43 +423,41 @@ __device__ __forceinline__ void store_chunk(const Geo &g, uint8_t *page, int gh,
     }
 }
 
-// The V rows of a q8_0 page that is dimension-major in its 64-token tiles: a workgroup's up
-// to 64 rows of one head are quantized by rows and turned in LDS.  Rows at positions that follow
-// each other (a prompt's) leave it as whole words, others byte by byte.
+// The V rows of a q8_0 page that is dimension-major in its 64-token tiles: a workgroup's up to
+// 64 rows of 64 dimensions (chunks c0 .. c0 + 7) of one head are quantized by rows, eight lanes
+// a row, and turned in LDS.  Rows at positions that follow each other (a prompt's) leave it as
+// whole words, others byte by byte.
 constexpr int kTurnRow = 68;                              // 64 bytes of a dimension, displaced by up to 3
-template <int HD>
 __device__ __forceinline__ void values_turned(const Geo &g, const qwfn_kv_view &v, const RowsArg &vv, const int32_t *seq_ids,
-                                              const int32_t *pos, int64_t row0, int64_t end, int h, uint8_t *lds) {
-    constexpr int LH = HD / 16, kRowsWave = 64 / LH;
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, e = lane % LH, tid = threadIdx.x;
+                                              const int32_t *pos, int64_t row0, int64_t end, int h, int c0, uint8_t *lds) {
+    const int lane = threadIdx.x & 63, tid = threadIdx.x, c = c0 + lane % 8, o0 = tid / 8;
     const int m = (int)(end - row0);
+    float x[2][8];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        load8(vv.data, vv.dtype, (row0 + min(o0 + 32 * k, m - 1)) * vv.row_stride + h * vv.head_stride + 8 * c, x[k]);
     const int t0 = pos[row0], s0 = seq_ids ? seq_ids[row0] : 0;
     bool run = t0 >= 0 && (int64_t)t0 + m <= (int64_t)g.pps * g.pt && s0 >= 0 && s0 < g.n_seq_view;
     if (tid < m) run = run && (int64_t)pos[row0 + tid] == (int64_t)t0 + tid && (!seq_ids || seq_ids[row0 + tid] == s0);
     run = __syncthreads_and(run);
     const int a = run ? t0 & 3 : 0;
-    for (int i = wv * kRowsWave; i < m; i += 4 * kRowsWave) {
-        const int o = i + lane / LH;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int o = o0 + 32 * k;
         const int64_t rr = row0 + min(o, m - 1);
         Dest d;
         const bool live = dest_of(g, v, seq_ids ? seq_ids[rr] : 0, pos[rr], false, d) && o < m;
         uint8_t *page = (uint8_t *)v.v_pages + (live ? (int64_t)d.page * g.page_bytes : 0);
+        uint16_t dh;
+        const uint2 w = quad_q8(x[k], g.variant, &dh);
+        if (live && (c & 3) == 0) *reinterpret_cast<uint16_t *>(page + scale_off(g, h, d.row, c / 4)) = dh;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int c = e + k * LH;
-            float x[8];
-            load8(vv.data, vv.dtype, rr * vv.row_stride + h * vv.head_stride + 8 * c, x);
-            uint16_t dh;
-            const uint2 w = quad_q8(x, g.variant, &dh);
-            if (live && (c & 3) == 0) *reinterpret_cast<uint16_t *>(page + scale_off(g, h, d.row, c / 4)) = dh;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint8_t b = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
-                if (run) {
-                    if (o < m) lds[(8 * c + j) * kTurnRow + a + o] = b;
-                } else if (live) {
-                    page[vquant_off(g, h, d.row, 8 * c + j)] = b;
-                }
+        for (int j = 0; j < 8; ++j) {
+            const uint8_t b = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
+            if (run) {
+                if (o < m) lds[(8 * (c - c0) + j) * kTurnRow + a + o] = b;
+            } else if (live) {
+                page[vquant_off(g, h, d.row, 8 * c + j)] = b;
             }
         }
     }
@@ -466,35 +468,38 @@ __device__ __forceinline__ void values_turned(const Geo &g, const qwfn_kv_view &
     const int tb = (t0 / g.pt + 1) * g.pt;                // the second page's first cell
     const int32_t pa = phys_page(g, v.page_table, s0, t0), pb = t0 + m > tb ? phys_page(g, v.page_table, s0, tb) : -1;
     uint8_t *va = (uint8_t *)v.v_pages + (int64_t)pa * g.page_bytes, *vb = (uint8_t *)v.v_pages + (int64_t)pb * g.page_bytes;
-    for (int i = tid; i < HD * 17; i += 256) {
-        const int dim = i / 17, k = i % 17, c0 = 4 * k - a, t = t0 + c0;
-        if (c0 >= m || (t < tb ? pa : pb) < 0) continue;
-        uint8_t *to = t < tb ? va + vquant_off(g, h, t - tb + g.pt, dim) : vb + vquant_off(g, h, t - tb, dim);
+    for (int i = tid; i < 64 * 17; i += 256) {
+        const int dim = i / 17, k = i % 17, o = 4 * k - a, t = t0 + o;
+        if (o >= m || (t < tb ? pa : pb) < 0) continue;
+        uint8_t *to = t < tb ? va + vquant_off(g, h, t - tb + g.pt, 8 * c0 + dim) : vb + vquant_off(g, h, t - tb, 8 * c0 + dim);
         const uint32_t w = *reinterpret_cast<const uint32_t *>(lds + dim * kTurnRow + 4 * k);
-        if (c0 >= 0 && c0 + 4 <= m) {
+        if (o >= 0 && o + 4 <= m) {
             *reinterpret_cast<uint32_t *>(to) = w;
         } else {
             for (int j = 0; j < 4; ++j)
-                if (c0 + j >= 0 && c0 + j < m) to[j] = (uint8_t)(w >> (8 * j));
+                if (o + j >= 0 && o + j < m) to[j] = (uint8_t)(w >> (8 * j));
         }
     }
 }
 
 // Q, K and V: grid (row blocks, a pass of the four waves each; groups of hq query heads, then of
-// hk key heads, then one a value head).  SZ: bytes of a source value.
+// hk key heads, then one a value head, or a 64-dimension part of one that is turned).  SZ: bytes of
+// a source value.
 template <int HD, int KT, bool IL, int SZ>
 __global__ void __launch_bounds__(256, 3)
 k_rope_append8(Geo g, qwfn_kv_view v, RopeArg rp, RowsArg q, RowsArg k, RowsArg vv, const float *q_norm,
                const float *k_norm, const int32_t *seq_ids, const int32_t *pos, int64_t n_rows, int n_q, int hq, int hk,
                RowsArg q_out) {
     constexpr int kRowsWave = 64 * 16 / HD;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[KT == QWFN_KV_Q8_0 ? HD * kTurnRow : 16];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[KT == QWFN_KV_Q8_0 ? 64 * kTurnRow : 16];
     const int qg = (n_q + hq - 1) / hq, kg = (g.Hkv + hk - 1) / hk;
     const int64_t b0 = (int64_t)blockIdx.x * (4 * kRowsWave);
     const int role = blockIdx.y, which = role < qg ? 0 : role < qg + kg ? 1 : 2;         // Q, K, V
     if (KT == QWFN_KV_Q8_0 && which == 2 && g.vdim) {
-        if (b0 % 64 == 0) values_turned<HD>(g, v, vv, seq_ids, pos, b0, min(b0 + 64, n_rows), role - qg - kg, lds);
-        return;                                                                          // (64 rows a workgroup)
+        const int i = role - qg - kg;                                                    // (64 rows, 64 dimensions)
+        if (b0 % 64 == 0)
+            values_turned(g, v, vv, seq_ids, pos, b0, min(b0 + 64, n_rows), i / (HD / 64), i % (HD / 64) * 8, lds);
+        return;
     }
     const RowsArg src = which == 0 ? q : which == 1 ? k : vv;
     const float *norm = which == 0 ? q_norm : which == 1 ? k_norm : nullptr;
@@ -596,7 +601,7 @@ hipError_t launch_rope_append(const Geo &g, const qwfn_kv_view &v, const RopeArg
         }
         const int rows = 4 * 64 * 16 / g.hd, blocks = (n_rows + rows - 1) / rows;
         const int hq = heads_a_wave(blocks, std::max(n_q, 1)), hk = std::min(heads_a_wave(blocks, g.Hkv), 2);
-        const unsigned roles = (n_q + hq - 1) / hq + (g.Hkv + hk - 1) / hk + g.Hkv;
+        const unsigned roles = (n_q + hq - 1) / hq + (g.Hkv + hk - 1) / hk + g.Hkv * (g.vdim ? g.hd / 64 : 1);
         const auto go = [&](auto kern) {
             hipLaunchKernelGGL(kern, dim3((unsigned)blocks, roles), dim3(256), 0, st, g, v, rp, q, k, vv, q_norm, k_norm,
                                seq_ids, pos, n_rows, n_q, hq, hk, q_out);
