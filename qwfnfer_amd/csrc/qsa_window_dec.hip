@@ -266,7 +266,10 @@ k_win_dec(Geo g, qwfn_kv_view v, WinArg wa, int parts, float *part_o, float2 *pa
     VTile<HD, KT, VD> vt;
     int32_t p;
     int i = next(part * 4 + w, p);
-    if (i < tl.n) {
+    // heads of 256 values: a tile's K, and after it its V, take the registers that the next tile
+    // would be held in
+    constexpr bool kAhead = HD < 256;
+    if (kAhead && i < tl.n) {
         const int t0 = tl.cell(i);
         load_k<HD, KT>(kt, quants(v.k_pages, p, t0), scales(v.k_pages, p, t0), hn, lg);
         load_v<HD, KT, VD>(vt, quants(v.v_pages, p, t0), scales(v.v_pages, p, t0), lane);
@@ -278,6 +281,7 @@ k_win_dec(Geo g, qwfn_kv_view v, WinArg wa, int parts, float *part_o, float2 *pa
         const bool more = in < tl.n;
         const int tn = more ? tl.cell(in) : 0;
         // ---- QK ----
+        if (!kAhead) load_k<HD, KT>(kt, quants(v.k_pages, p, t0), scales(v.k_pages, p, t0), hn, lg);
         float x[4][4];
 #pragma unroll
         for (int cg = 0; cg < 4; ++cg) {
@@ -302,7 +306,8 @@ k_win_dec(Geo g, qwfn_kv_view v, WinArg wa, int parts, float *part_o, float2 *pa
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[cg][j] = (LOC ? ror8_add(a[j]) : a[j]) * qscale;
         }
-        if (more) load_k<HD, KT>(kt, quants(v.k_pages, pn, tn), scales(v.k_pages, pn, tn), hn, lg);
+        if (!kAhead) load_v<HD, KT, VD>(vt, quants(v.v_pages, p, t0), scales(v.v_pages, p, t0), lane);
+        if (kAhead && more) load_k<HD, KT>(kt, quants(v.k_pages, pn, tn), scales(v.k_pages, pn, tn), hn, lg);
         // ---- the tile's edges ----
         uint32_t keep = 0xFFFFFFFFu;                    // F16 V: cells 2 p, 2 p + 1 of the staging lane
         if (!tl.whole(i, len)) {
@@ -392,8 +397,9 @@ k_win_dec(Geo g, qwfn_kv_view v, WinArg wa, int parts, float *part_o, float2 *pa
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
-        if (more) load_v<HD, KT, VD>(vt, quants(v.v_pages, pn, tn), scales(v.v_pages, pn, tn), lane);
+        if (kAhead && more) load_v<HD, KT, VD>(vt, quants(v.v_pages, pn, tn), scales(v.v_pages, pn, tn), lane);
         i = in;
+        p = pn;
     }
 
     // ---- the four waves' states into one ----
