@@ -482,7 +482,8 @@ typedef struct qwfn_rows {
  * way: the transpose of the rotation (over mscale^2, its inverse), which is also the
  * gradient of unnormed rows.  head_dim 1 .. 512, rope_dim <= head_dim.  dst is src itself (same
  * pointer, type and strides) or apart from it: QWFN_EINVAL when they overlap
- * otherwise.  Head rows of dst must not overlap each other.                    */
+ * otherwise.  Head rows of dst must not overlap each other.  QWFN_ERANGE past
+ * 2^26 - 4 head rows a call (here and below).                                 */
 int qwfn_rope_rows(const qwfn_rope *rope, const qwfn_rows *src, const float *norm, const int32_t *pos,
                    int32_t n_rows, int32_t n_heads, int32_t head_dim, int32_t inverse, const qwfn_rows *dst,
                    void *stream);

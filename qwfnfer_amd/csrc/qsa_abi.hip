@@ -1145,6 +1145,9 @@ int qwfn_idx_sparse_attn_prefill(const qwfn_qsa_shape *shape, const qwfn_kv_view
 
 // ---- rotary positions ----
 
+// Head rows of a call: a wave each, and a launch has fewer than 2^32 threads.
+static constexpr int64_t kMaxHeadRows = (1 << 26) - 4;
+
 static size_t dtype_size(int32_t t) { return t == QWFN_SRC_F32 ? 4 : 2; }
 
 static int check_dtype(const char *what, int32_t t) {
@@ -1208,8 +1211,8 @@ int qwfn_rope_rows(const qwfn_rope *rope, const qwfn_rows *src, const float *nor
     if (n_rows < 1 || n_heads < 1) return fail(QWFN_EINVAL, "rope_rows: n_rows %d or n_heads %d < 1", n_rows, n_heads);
     if (head_dim < 1 || head_dim > kRopeMaxDim)
         return fail(QWFN_EINVAL, "rope_rows: head_dim %d outside [1, %d]", head_dim, kRopeMaxDim);
-    if ((int64_t)n_rows * n_heads > INT32_MAX)
-        return fail(QWFN_ERANGE, "rope_rows: more than %d head rows", INT32_MAX);
+    if ((int64_t)n_rows * n_heads > kMaxHeadRows)
+        return fail(QWFN_ERANGE, "rope_rows: more than %lld head rows", (long long)kMaxHeadRows);
     RopeArg rp;
     RowsArg s, d;
     int rc;
@@ -1234,8 +1237,8 @@ int qwfn_kv_append_rope(const qwfn_qsa_shape *shape, const qwfn_kv_view *view, c
     int rc = make_geo(shape, view, &g);
     if (rc) return rc;
     if (n_rows < 1) return fail(QWFN_EINVAL, "append_rope: n_rows %d < 1", n_rows);
-    if ((int64_t)n_rows * (g.H + 2 * g.Hkv) > INT32_MAX)
-        return fail(QWFN_ERANGE, "append_rope: more than %d head rows", INT32_MAX);
+    if ((int64_t)n_rows * (g.H + 2 * g.Hkv) > kMaxHeadRows)
+        return fail(QWFN_ERANGE, "append_rope: more than %lld head rows", (long long)kMaxHeadRows);
     RopeArg rp;
     RowsArg ka, va, qa{nullptr, 0, 0, 0}, qo{nullptr, 0, 0, 0};
     if ((rc = make_rope("append_rope", rope, g.hd, 0, &rp)) ||
@@ -1276,7 +1279,8 @@ static int check_window(const char *what, const Geo &g, const WinPlan &p) {
     if (p.max_seq_len > INT32_MAX / 2) return fail(QWFN_ERANGE, "%s: max_seq_len %d", what, p.max_seq_len);
     if ((int64_t)p.n_seq * g.Hkv > kMaxCounters)
         return fail(QWFN_ERANGE, "%s: n_seq * n_head_kv = %lld exceeds %d", what, (long long)p.n_seq * g.Hkv, kMaxCounters);
-    if ((int64_t)p.n_rows * g.H > INT32_MAX) return fail(QWFN_ERANGE, "%s: n_rows * n_head exceeds %d", what, INT32_MAX);
+    if ((int64_t)p.n_rows * g.H > kMaxHeadRows)
+        return fail(QWFN_ERANGE, "%s: n_rows * n_head exceeds %lld", what, (long long)kMaxHeadRows);
     return QWFN_OK;
 }
 

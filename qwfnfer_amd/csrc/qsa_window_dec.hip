@@ -16,6 +16,13 @@
 // cost no second MFMA.
 // Weights are e^(s - r) with r at least max(s) + log2(V scale bound) - 14: the fp16
 // products stay below 2^14 and keep 22 bits down to 2^-38 of the largest.
+//
+// Measured (MI355X): 64 sequences of up to 4,160 cells, q8_0, 2 x 128 KV heads: 39.7 us for 135 MB,
+// 3.4 TB/s of the 5.2 that a large copy reaches.  The waves' tiles come in whole rounds (up to 5 for
+// 3.8 on average) and a round waits for its loads: VALU active 34 %, 1,045 instructions a tile.
+// Workgroups for two a CU: three, four and six a CU measured 46, 47 and 50 us.  One sequence over
+// 1,024 cells: 8.5 us, a chain of dependent loads (length, page, tile), one tile a wave, then the
+// merge's 3.2 us.  A tile held ahead in registers needs heads of at most 128 values.
 #include <hip/hip_runtime.h>
 
 #include "qsa_append.h"

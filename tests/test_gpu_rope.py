@@ -102,6 +102,14 @@ def test_rows_counts(n, heads):
     check_rows(qsa.rope_rows(rope, x, pos), turned(rope, x, np_of(pos)), torch.bfloat16)
 
 
+def test_rows_of_many_heads():
+    """More groups of heads than a grid's second dimension holds."""
+    rope = rope_of(64)
+    x = torch.randn(2, 300000, 64, device="cuda").half()
+    pos = torch.tensor([7, 70000], dtype=torch.int32, device="cuda")
+    check_rows(qsa.rope_rows(rope, x, pos), turned(rope, x, np_of(pos)), torch.float16)
+
+
 def test_rows_extreme_positions():
     rope = rope_of(128)
     x = torch.randn(6, 2, 128, device="cuda")

@@ -87,6 +87,8 @@ def test_rope_rows_refusals(kw):
 
 def test_rope_rows_too_many():
     assert _rope_rows(n=1 << 30, heads=4, src=_rows(rs=512), dst=_rows(data=1 << 60, rs=512)) == ERANGE
+    assert _rope_rows(n=1 << 24, heads=4, src=_rows(rs=512), dst=_rows(data=1 << 60, rs=512)) == ERANGE
+    assert _append(n=1 << 22) == ERANGE
 
 
 def _view(pps=4, n_seq=1, nphys=4, k=4096):
@@ -142,6 +144,7 @@ def test_window_prefill_refusals():
     assert _attn(False, n_rows=0) == EINVAL
     assert _attn(False, max_q=0) == EINVAL
     assert _attn(False, n_rows=1 << 28) == ERANGE
+    assert _attn(False, n_rows=1 << 22) == ERANGE
 
 
 def test_window_workspace_sizes():
