@@ -322,6 +322,33 @@ def test_append_non_finite_rows(kv):
         assert torch.equal(a.k_pages, b.k_pages) and torch.equal(a.v_pages, b.v_pages)
 
 
+@pytest.mark.parametrize("kv", [0, 1, 2])
+@pytest.mark.parametrize("types,off", [(("f32", "bf16", "bf16"), 0), (("bf16", "f16", "f32"), 0), (("bf16", "bf16", "bf16"), 3),
+                                       (("f16", "f32", "f32"), 1)])
+def test_append_mixed_types_and_alignment(kv, types, off):
+    """Sources of several types, rows that begin at an odd element, a float16 q_out with gaps between heads."""
+    cfg = qsa.QsaConfig(kv_type=kv)
+    rope = rope_of(128)
+    gen = torch.Generator(device="cuda").manual_seed(off)
+    n = 90
+
+    def source(heads, t):
+        buf = torch.empty(n * heads * 160 + 8, device="cuda", dtype=TYPES[t])
+        x = buf[off:off + n * heads * 160].view(n, heads, 160)[:, :, :128]
+        x.copy_(rows(gen, n, heads, 128, TYPES[t]))
+        return x
+
+    q, k, v = (source(h, t) for h, t in zip((16, 2, 2), types))
+    pos = torch.arange(5, 5 + n, dtype=torch.int32, device="cuda")
+    a, b = (qsa.KvCache.allocate(cfg, 1, 1) for _ in range(2))
+    q_out = torch.zeros(n, 16, 192, dtype=torch.float16, device="cuda")[:, :, 32:160]
+    assert qsa.append_rope(a, rope, k, v, pos, q=q, q_out=q_out) is q_out
+    check_rows(q_out, turned(rope, q, np_of(pos)), torch.float16)
+    turned_k = torch.from_numpy(turned(rope, k, np_of(pos)).astype(np.float32)).cuda()
+    qsa.append_q8_0(b, turned_k, v.float().contiguous(), pos)
+    assert torch.equal(a.k_pages, b.k_pages) and torch.equal(a.v_pages, b.v_pages)
+
+
 def test_append_captured_and_replayed():
     """One graph, replayed with new rows and positions between eager work, each replay against eager calls."""
     cfg = qsa.QsaConfig()

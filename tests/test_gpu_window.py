@@ -493,6 +493,28 @@ def test_on_another_stream():
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("kv", [0, 2])
+def test_pages_past_32_bits(kv):
+    """Pages more than 4 GiB into their pool: the bytes and results of the same rows in a small one."""
+    cfg = config("base", kv)
+    far = 2 ** 32 // cfg.page_bytes() + 2
+    rope = qsa.Rope(qsa.RopeConfig(rope_dim=128))
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(700, 20, 128, device="cuda", generator=gen).bfloat16()
+    pos = torch.arange(700, dtype=torch.int32, device="cuda")
+    start, lens = (torch.tensor(a, dtype=torch.int32, device="cuda") for a in ([0, 100], [700]))
+    got = []
+    for table, phys in ([[0, 1, 2]], 3), ([[far, far + 2, far + 1]], far + 3):
+        c = qsa.KvCache.allocate(cfg, 1, 3, page_table=torch.tensor(table, dtype=torch.int32), n_phys_pages=phys)
+        q = qsa.append_rope(c, rope, x[:, 16:18], x[:, 18:], pos, q=x[:, :16])
+        ws = qsa.Workspace.for_window(cfg, 1, 768, 300, 4, n_rows=100, max_q=100)
+        got.append((qsa.window_attn_decode(c, q[-1:].contiguous(), lens, 768, 300, ws, sink_tokens=4),
+                    qsa.window_attn_prefill(c, q[600:].contiguous(), start, lens, 100, 768, 300, ws, sink_tokens=4)))
+        assert qsa.read_status(c) == 0 and got[-1][0].any()
+        del c
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 # ---- a run of them, as a program makes it ------------------------------------------
 
 @pytest.mark.parametrize("kv", [0, 1, 2])
