@@ -915,6 +915,7 @@ class Rope:
             raise ValueError(f"turns has {turns.numel()} values, expected {cfg.rope_dim // 2}")
         self.cfg = cfg
         self.turns = turns.to(device=device, dtype=torch.float64).contiguous()
+        self.device = self.turns.get_device()
         self._c = RopeStruct(cfg.rope_dim, _lib.ROPE_HALF if cfg.layout == "half" else _lib.ROPE_INTERLEAVED,
                              self.turns.data_ptr(), cfg.scale(), cfg.norm_eps)
 
@@ -929,7 +930,7 @@ def _rows(t: torch.Tensor, name: str, n_rows: int, n_heads: int, head_dim: int, 
     """The C struct of head rows [n_rows, n_heads, head_dim] with any row and head stride, on a device."""
     # the usual case in one expression; what fails it is told apart below (a struct packed into bytes
     # and the device by its number: 1 us a tensor less than a ctypes struct and torch.device)
-    if isinstance(t, torch.Tensor) and t.shape == (n_rows, n_heads, head_dim) and t.get_device() == device and device >= 0:
+    if isinstance(t, torch.Tensor) and t.shape == (n_rows, n_heads, head_dim) and t.get_device() == device >= 0:
         dtype = _DTYPES.get(t.dtype)
         rs, hs, one = t.stride()
         if dtype is not None and (one == 1 or head_dim == 1):
@@ -984,7 +985,8 @@ def rope_rows(rope: Rope, x: torch.Tensor, pos: torch.Tensor, norm: Optional[tor
     _need(pos, "pos", torch.int32, n)
     if norm is not None:
         _need(norm, "norm", torch.float32, hd)
-    _beside(dev, pos=pos, norm=norm, turns=rope.turns)
+    if not (pos.get_device() == dev == rope.device and (norm is None or norm.get_device() == dev)):
+        _beside(dev, pos=pos, norm=norm, turns=rope.turns)
     _call_on(dev, stream, "qwfn_rope_rows", rope.c_ref(), src, _ptr(norm), pos.data_ptr(), n, heads, hd,
              1 if inverse else 0, dst)
     return out
@@ -1021,7 +1023,9 @@ def append_rope(cache: KvCache, rope: Rope, k: torch.Tensor, v: torch.Tensor, po
         _need(k_norm, "k_norm", torch.float32, hd)
     if q_norm is not None:
         _need(q_norm, "q_norm", torch.float32, hd)
-    _beside(dev, pos=pos, seq_ids=seq_ids, k_norm=k_norm, q_norm=q_norm, turns=rope.turns)
+    if not (pos.get_device() == dev == rope.device and (seq_ids is None or seq_ids.get_device() == dev) and
+            (k_norm is None or k_norm.get_device() == dev) and (q_norm is None or q_norm.get_device() == dev)):
+        _beside(dev, pos=pos, seq_ids=seq_ids, k_norm=k_norm, q_norm=q_norm, turns=rope.turns)
     _call_on(dev, stream, "qwfn_kv_append_rope", C.byref(cache.c_shape()), C.byref(cache.view()), rope.c_ref(),
              kr, vr, _ptr(k_norm), _ptr(seq_ids), pos.data_ptr(), n, qr, _ptr(q_norm), qo)
     return q_out
@@ -1041,7 +1045,8 @@ def _window_rows(cache: KvCache, q: torch.Tensor, n_rows: Optional[int], out: Op
     if out is None:
         out = torch.empty((n_rows, cfg.n_head, cfg.head_dim), dtype=q.dtype, device=q.device)
     _need(out, "out", q.dtype, n_rows * width)
-    _beside(dev, q=q, out=out, ws=ws.buf)
+    if not (q.get_device() == out.get_device() == ws.buf.get_device() == dev):
+        _beside(dev, q=q, out=out, ws=ws.buf)
     return dtype, n_rows, out, dev
 
 
@@ -1057,7 +1062,8 @@ def window_attn_decode(cache: KvCache, q: torch.Tensor, seq_len: torch.Tensor, m
     n_seq = seq_len.numel()
     _need(seq_len, "seq_len", torch.int32)
     dtype, _, out, dev = _window_rows(cache, q, n_seq, out, ws)
-    _beside(dev, seq_len=seq_len)
+    if seq_len.get_device() != dev:
+        _beside(dev, seq_len=seq_len)
     if n_seq == 0:
         return out
     _call_on(dev, stream, "qwfn_window_attn_decode", C.byref(cache.c_shape()), C.byref(cache.view()), q.data_ptr(),
