@@ -16,10 +16,10 @@
 // over several heads with them.  k_rope_rows and k_rope_append take everything
 // else, a wave a head row through LDS (8,192 x 16 rows 73 us).
 //
-// Measured (MI355X): 8,192 x 16 bfloat16 rows of 128, normed: 18.2 us, 3.7 TB/s of the 5.2 that a
+// Measured (MI355X): 8,192 x 16 bfloat16 rows of 128, normed: 18.9 us by the kernel, 3.6 TB/s of the 5.2 that a
 // large copy reaches; 1,628 vector instructions a wave of 8 rows x 4 heads are 60 % of the time, a
 // fourth of them cos and sin.  8,000 rows of K and V into q8_0: 21.7 us (a wave's chain of loads, norm
-// and division), their 16 query heads beside it 28.8 us for 98 MB.  64 single rows 5.8 us, one 5.0.
+// and division), their 16 query heads beside it 27.0 us for 98 MB.  64 single rows 5.8 us, one 5.0.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -159,13 +159,9 @@ struct Place {
 
 // A lane's cos and sin: IL: of chunk a's four pairs and b's; HALF: of the eight pairs of a and b.
 template <int HD, bool IL>
-__device__ __forceinline__ void place_cs(const Place<HD, IL> &pl, const RopeArg &rp, int pos, double2 (&cs)[8]) {
-    double p = (double)pos, f[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {                         // (every load before the first is used)
-        const bool on = k < 4 || !IL ? pl.ta : pl.tb;
-        f[k] = rp.turns[on ? IL ? 4 * (k < 4 ? pl.a : pl.b) + (k & 3) : 8 * pl.a + k : 0];
-    }
+__device__ __forceinline__ void place_cs(const Place<HD, IL> &pl, const RopeArg &rp, int pos, const double (&f)[8],
+                                         double2 (&cs)[8]) {
+    double p = (double)pos;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         cs[k] = make_double2(0.0, 0.0);
@@ -292,30 +288,45 @@ struct Raw {
     }
 };
 
+// What a lane reads before it knows more than its row: the first head's chunks, the norm's weights
+// and the frequencies of its pairs, all in flight together (and before a page is looked up).
+template <int HD, bool IL, int SZ>
+struct Front {
+    Raw<SZ> raw;
+    float w[16];
+    double f[8];
+    __device__ __forceinline__ Front(const RopeArg &rp, const Place<HD, IL> &pl, const RowsArg &src, const float *norm,
+                                     int64_t rr, int h0) {
+        raw.load(src, rr * src.row_stride + h0 * src.head_stride, pl.a, pl.b);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const bool on = k < 4 || !IL ? pl.ta : pl.tb;
+            f[k] = rp.turns[on ? IL ? 4 * (k < 4 ? pl.a : pl.b) + (k & 3) : 8 * pl.a + k : 0];
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) w[k] = 1.0f;
+        if (norm) {
+            load8(norm, QWFN_SRC_F32, 8 * pl.a, w);
+            load8(norm, QWFN_SRC_F32, 8 * pl.b, w + 8);
+        }
+    }
+};
+
 // Rows of HD values in 16-byte pieces: a wave 64 / LH rows at a time, heads h0 .. h1 - 1 with
 // one cos and sin; put(h, x) takes the lane's 16 results of head h.
 template <int HD, bool IL, int SZ, class Put>
-__device__ __forceinline__ void heads8(const RopeArg &rp, const Place<HD, IL> &pl, const RowsArg &src, const float *norm,
-                                       int64_t rr, int pos, int h0, int h1, Put put) {
+__device__ __forceinline__ void heads8(const RopeArg &rp, const Place<HD, IL> &pl, const RowsArg &src, bool norm,
+                                       Front<HD, IL, SZ> &in, int64_t rr, int pos, int h0, int h1, Put put) {
     const int64_t at = rr * src.row_stride;
-    Raw<SZ> next;
-    next.load(src, at + h0 * src.head_stride, pl.a, pl.b);
-    float w[16];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) w[k] = 1.0f;
-    if (norm) {
-        load8(norm, QWFN_SRC_F32, 8 * pl.a, w);
-        load8(norm, QWFN_SRC_F32, 8 * pl.b, w + 8);
-    }
     double2 cs[8];
-    place_cs(pl, rp, pos, cs);
+    place_cs(pl, rp, pos, in.f, cs);
     for (int h = h0; h < h1; ++h) {
         float x[16];
-        next.values(src.dtype, x);
+        in.raw.values(src.dtype, x);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) asm("" : "+v"(w[k]));            // (its 64-bit form is not held over the loop)
-        if (h + 1 < h1) next.load(src, at + (h + 1) * src.head_stride, pl.a, pl.b);
-        turn16(pl, x, norm != nullptr, w, cs, rp.eps);
+        for (int k = 0; k < 16; ++k) asm("" : "+v"(in.w[k]));         // (its 64-bit form is not held over the loop)
+        if (h + 1 < h1) in.raw.load(src, at + (h + 1) * src.head_stride, pl.a, pl.b);
+        turn16(pl, x, norm, in.w, cs, rp.eps);
         put(h, x);
     }
 }
@@ -330,7 +341,8 @@ k_rope_rows8(RopeArg rp, RowsArg src, const float *norm, const int32_t *pos, int
     if (row0 >= n_rows) return;
     const Place<HD, IL> pl(lane, rp.rd);
     const int64_t r = row0 + lane / pl.LH, rr = min(r, n_rows - 1), to = rr * dst.row_stride;
-    heads8<HD, IL, SZ>(rp, pl, src, norm, rr, pos[rr], h0, min(h0 + hg, heads), [&](int h, const float *x) {
+    Front<HD, IL, SZ> in(rp, pl, src, norm, rr, h0);
+    heads8<HD, IL, SZ>(rp, pl, src, norm != nullptr, in, rr, pos[rr], h0, min(h0 + hg, heads), [&](int h, const float *x) {
         if (r >= n_rows) return;
         store8(dst.data, dst.dtype, to + h * dst.head_stride + 8 * pl.a, x);
         store8(dst.data, dst.dtype, to + h * dst.head_stride + 8 * pl.b, x + 8);
@@ -515,15 +527,16 @@ k_rope_append8(Geo g, qwfn_kv_view v, RopeArg rp, RowsArg q, RowsArg k, RowsArg 
     const int64_t row0 = b0 + (threadIdx.x >> 6) * kRowsWave;
     if (row0 >= n_rows) return;
     const int64_t r = row0 + lane / pl.LH, rr = min(r, n_rows - 1);
-    const int t = pos[rr];
+    const int t = pos[rr], seq = seq_ids ? seq_ids[rr] : 0;
+    Front<HD, IL, SZ> in(rp, pl, src, norm, rr, h0);
     Dest d{0, 0};
     bool live = r < n_rows;
     if (which) {
         const bool report = live && which == 1 && h0 == 0 && pl.e == 0;
-        live = dest_of(g, v, seq_ids ? seq_ids[rr] : 0, t, report, d) && live;
+        live = dest_of(g, v, seq, t, report, d) && live;
     }
     uint8_t *page = (uint8_t *)(which == 1 ? v.k_pages : v.v_pages) + (live ? (int64_t)d.page * g.page_bytes : 0);
-    heads8<HD, IL, SZ>(rp, pl, src, norm, rr, t, h0, h1, [&](int h, const float *x) {
+    heads8<HD, IL, SZ>(rp, pl, src, norm != nullptr, in, rr, t, h0, h1, [&](int h, const float *x) {
         if (which) {
             store_chunk<KT>(g, page, h, d.row, pl.a, x, live);
             store_chunk<KT>(g, page, h, d.row, pl.b, x + 8, live);
