@@ -18,7 +18,7 @@
 //
 // Measured (MI355X): 8,192 x 16 bfloat16 rows of 128, normed: 18.9 us by the kernel, 3.6 TB/s of the 5.2 that a
 // large copy reaches; 1,628 vector instructions a wave of 8 rows x 4 heads are 60 % of the time, a
-// fourth of them cos and sin.  8,000 rows of K and V into q8_0: 21.7 us (a wave's chain of loads, norm
+// fourth of them cos and sin.  8,000 rows of K and V into q8_0: 20.4 us (a wave's chain of loads, norm
 // and division), their 16 query heads beside it 27.0 us for 98 MB.  64 single rows 5.8 us, one 5.0.
 #include <hip/hip_runtime.h>
 
@@ -458,12 +458,22 @@ __device__ __forceinline__ void values_turned(const Geo &g, const qwfn_kv_view &
     if (tid < m) run = run && (int64_t)pos[row0 + tid] == (int64_t)t0 + tid && (!seq_ids || seq_ids[row0 + tid] == s0);
     run = __syncthreads_and(run);
     const int a = run ? t0 & 3 : 0;
+    // a run's rows lie in one page or two: looked up once, not a row (tb: the second's first cell)
+    int tb = 0;
+    int32_t pa = -1, pb = -1;
+    if (run) {
+        tb = (t0 / g.pt + 1) * g.pt;
+        pa = phys_page(g, v.page_table, s0, t0);
+        if (t0 + m > tb) pb = phys_page(g, v.page_table, s0, tb);
+    }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        const int o = o0 + 32 * k;
+        const int o = o0 + 32 * k, t = t0 + o;
         const int64_t rr = row0 + min(o, m - 1);
-        Dest d;
-        const bool live = dest_of(g, v, seq_ids ? seq_ids[rr] : 0, pos[rr], false, d) && o < m;
+        Dest d{t < tb ? pa : pb, t < tb ? t - tb + g.pt : t - tb};
+        bool live = o < m;
+        if (run) live = live && d.page >= 0;
+        else live = dest_of(g, v, seq_ids ? seq_ids[rr] : 0, pos[rr], false, d) && live;
         uint8_t *page = (uint8_t *)v.v_pages + (live ? (int64_t)d.page * g.page_bytes : 0);
         uint16_t dh;
         const uint2 w = quad_q8(x[k], g.variant, &dh);
@@ -480,10 +490,7 @@ __device__ __forceinline__ void values_turned(const Geo &g, const qwfn_kv_view &
     }
     if (!run) return;
     __syncthreads();
-    // word k of a dimension: cells t0 - a + 4 k .. + 3, which lie in one tile; the rows lie in one
-    // page or two
-    const int tb = (t0 / g.pt + 1) * g.pt;                // the second page's first cell
-    const int32_t pa = phys_page(g, v.page_table, s0, t0), pb = t0 + m > tb ? phys_page(g, v.page_table, s0, tb) : -1;
+    // word k of a dimension: cells t0 - a + 4 k .. + 3, which lie in one tile
     uint8_t *va = (uint8_t *)v.v_pages + (int64_t)pa * g.page_bytes, *vb = (uint8_t *)v.v_pages + (int64_t)pb * g.page_bytes;
     for (int i = tid; i < 64 * 17; i += 256) {
         const int dim = i / 17, k = i % 17, o = 4 * k - a, t = t0 + o;
